@@ -422,6 +422,45 @@ TLC_API int32_t tlc_attention_decode_static(void *stream, const void *q_dev, con
  * keys there, else 0; the note is cleared.  Allocates nothing. */
 TLC_API int32_t tlc_attention_decode_static_status(void *stream, int32_t *clamped_out);
 
+/* ---- 8-bit KV cache --------------------------------------------------------- */
+
+/* A KV cache in half the bytes (no counterpart in the reference, whose KVCache, src/model/llama.rs:51-116, is
+ * f16): 64 consecutive positions of a KV head of a sequence and layer form a block; a full block is held as
+ * 8-bit codes rint(127 x / a) with one scale a / 127, a the largest magnitude among its 64 * head_dim
+ * values, K and V apart.  The rows of a block that is not full yet are held in f16 as they came, so a value is
+ * rounded once and does not depend on how many rows came with each call.  The cache holds finite values: NaN
+ * becomes zero, an infinity +-65504.  head_dim is 64 or 128.  It keeps, per layer and sequence, how many
+ * rows it holds, on the device.  A cache belongs to the context that made it (others are refused). */
+typedef struct tlc_kvcache8 tlc_kvcache8;
+TLC_API int32_t tlc_kvcache8_create(tlc_ctx *ctx, int32_t n_layers, int32_t max_batch, int32_t max_seq,
+                                    int32_t n_kv_heads, int32_t head_dim, tlc_kvcache8 **out);
+TLC_API int32_t tlc_kvcache8_destroy(tlc_kvcache8 *cache);
+/* tlc_kvcache_append for the 8-bit cache.  k/v: [m, n_kv_heads, head_dim] f16, 16-byte aligned.
+ * positions_dev == NULL: m consecutive tokens of `sequence` from pos_offset on; otherwise row r is the new
+ * token of sequence `sequence + r` at positions_dev[r], and a negative position means no row for it.  Rows
+ * join at the end, or at an earlier position: the rows behind it are then gone, and rows in front of it
+ * that lie in a full block come back as the values they were held as.  A position past the end of a
+ * sequence, or past max_seq, is skipped and reported as TLC_ERR_INDEX by the next tlc_synchronize. */
+TLC_API int32_t tlc_kvcache8_append(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t layer, const void *k_dev,
+                                    const void *v_dev, int32_t m, int32_t sequence, int32_t pos_offset,
+                                    const int32_t *positions_dev);
+/* get_k / get_v (src/model/llama.rs:101-116): what the cache holds of rows [first, first + n) of n_sequences
+ * sequences from `sequence` on, as f16 [n_sequences, n, n_kv_heads, head_dim] each (16-byte aligned); zeros
+ * for rows a sequence does not have. */
+TLC_API int32_t tlc_kvcache8_rows(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t layer, int32_t sequence,
+                                  int32_t n_sequences, int32_t first, int32_t n, void *k_out_dev,
+                                  void *v_out_dev);
+/* tlc_attention over the 8-bit cache, for sequences `sequence` .. `sequence + batch - 1`; any number of query
+ * heads per KV head; q and out 16-byte aligned.  Scores, softmax and sums are f32.  With positions_dev a
+ * negative position marks an idle slot, whose output rows are zeros.  A query at a position whose key the cache
+ * does not hold (or at or past max_keys) sees the keys there are, and the next tlc_synchronize reports
+ * TLC_ERR_INDEX.  Allocates nothing, except on the first prompt long enough for the tensor-memory kernel (an
+ * f16 image of one sequence and layer): make that call before a stream capture. */
+TLC_API int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t layer, const void *q_dev,
+                               void *out_dev, int32_t batch, int32_t n_queries, int32_t n_heads,
+                               int32_t sequence, int32_t q_pos0, const int32_t *positions_dev,
+                               int32_t max_keys, float scale);
+
 /* ---- GGUF models ----------------------------------------------------------- */
 
 /* load_model(path) (src/interpreter/builtin_model.rs:106-131 -> Model::load,
@@ -548,6 +587,17 @@ TLC_API int32_t tlc_temperature_sample(tlc_ctx *ctx, const void *logits_dev, int
  * gather + sampling); tokens and positions are left untouched unless parts == 7. */
 TLC_API int32_t tlc_llama_decode_enqueue_parts(tlc_llama *l, int32_t batch, int32_t steps,
                                                int32_t parts);
+/* How likely the model found given tokens (no counterpart in the reference): per row of logits_dev [rows, vocab]
+ * f16 the log-softmax of the row's target, the entropy of its distribution (nats) and the top_k (0 .. 32)
+ * likeliest tokens with their log probabilities, equal logits in the order of their ids.  Logits that are not
+ * finite carry no probability, as in tlc_softmax.  targets_dev: int32 [rows]; -1 means no target (0 is
+ * written).  Outputs f32 [rows], f32 [rows], int32 and f32 [rows, top_k]; any of the first two may be NULL,
+ * and targets_dev with logprobs_dev.  Where a row has fewer than top_k finite logits the rest are id -1 and -inf;
+ * a row without any has log probability -inf and entropy 0.  A target outside [-1, vocab) gives NaN, and the
+ * next tlc_synchronize reports TLC_ERR_INDEX. */
+TLC_API int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int32_t rows, int32_t vocab,
+                                   const int32_t *targets_dev, int32_t top_k, float *logprobs_dev,
+                                   float *entropy_dev, int32_t *top_ids_dev, float *top_logprobs_dev);
 /* ---- tensor parallelism ----------------------------------------------------- */
 
 /* No counterpart in the reference (it has no multi-GPU code).  One process per

@@ -18,7 +18,7 @@ PRIM = {"int32_t": "i32", "int64_t": "i64", "uint32_t": "u32", "uint64_t": "u64"
 
 
 def camel(name: str) -> str:
-    special = {"qtensor": "QTensor", "kvcache": "KvCache"}
+    special = {"qtensor": "QTensor", "kvcache": "KvCache", "kvcache8": "KvCache8"}
     return "Tlc" + "".join(special.get(p, p.capitalize()) for p in name[4:].split("_"))
 
 

@@ -18,6 +18,8 @@ pub struct TlcGguf { _private: [u8; 0] }
 #[repr(C)]
 pub struct TlcKvCache { _private: [u8; 0] }
 #[repr(C)]
+pub struct TlcKvCache8 { _private: [u8; 0] }
+#[repr(C)]
 pub struct TlcLlama { _private: [u8; 0] }
 #[repr(C)]
 pub struct TlcModel { _private: [u8; 0] }
@@ -170,6 +172,18 @@ extern "C" {
                                        head_dim: i32, max_seq: i32, positions_dev: *const i32,
                                        max_keys: i32, scale: f32) -> i32;
     pub fn tlc_attention_decode_static_status(stream: *mut c_void, clamped_out: *mut i32) -> i32;
+    pub fn tlc_kvcache8_create(ctx: *mut TlcCtx, n_layers: i32, max_batch: i32, max_seq: i32,
+                               n_kv_heads: i32, head_dim: i32, out: *mut *mut TlcKvCache8) -> i32;
+    pub fn tlc_kvcache8_destroy(cache: *mut TlcKvCache8) -> i32;
+    pub fn tlc_kvcache8_append(ctx: *mut TlcCtx, cache: *mut TlcKvCache8, layer: i32, k_dev: *const c_void,
+                               v_dev: *const c_void, m: i32, sequence: i32, pos_offset: i32,
+                               positions_dev: *const i32) -> i32;
+    pub fn tlc_kvcache8_rows(ctx: *mut TlcCtx, cache: *mut TlcKvCache8, layer: i32, sequence: i32,
+                             n_sequences: i32, first: i32, n: i32, k_out_dev: *mut c_void,
+                             v_out_dev: *mut c_void) -> i32;
+    pub fn tlc_attention8(ctx: *mut TlcCtx, cache: *mut TlcKvCache8, layer: i32, q_dev: *const c_void,
+                          out_dev: *mut c_void, batch: i32, n_queries: i32, n_heads: i32, sequence: i32,
+                          q_pos0: i32, positions_dev: *const i32, max_keys: i32, scale: f32) -> i32;
     pub fn tlc_model_load_gguf(ctx: *mut TlcCtx, path: *const c_char, tp_rank: i32, tp_size: i32,
                                out: *mut *mut TlcModel) -> i32;
     pub fn tlc_weight_cache_open(ctx: *mut TlcCtx, path: *const c_char, capacity: i64,
@@ -214,6 +228,9 @@ extern "C" {
     pub fn tlc_temperature_sample(ctx: *mut TlcCtx, logits_dev: *const c_void, rows: i32, vocab: i32,
                                   temperature: f32, uniforms_host: *const f32, ids_host: *mut i32) -> i32;
     pub fn tlc_llama_decode_enqueue_parts(l: *mut TlcLlama, batch: i32, steps: i32, parts: i32) -> i32;
+    pub fn tlc_token_logprobs(ctx: *mut TlcCtx, logits_dev: *const c_void, rows: i32, vocab: i32,
+                              targets_dev: *const i32, top_k: i32, logprobs_dev: *mut f32,
+                              entropy_dev: *mut f32, top_ids_dev: *mut i32, top_logprobs_dev: *mut f32) -> i32;
     pub fn tlc_comm_unique_id(out128: *mut c_void) -> i32;
     pub fn tlc_comm_init(ctx: *mut TlcCtx, id128: *const c_void, rank: i32, world: i32,
                          out: *mut *mut TlcComm) -> i32;

@@ -112,6 +112,11 @@ PROTOTYPES = {
     "tlc_attention": (i32, [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, i32, f32]),
     "tlc_attention_decode_static": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i32, f32]),
     "tlc_attention_decode_static_status": (i32, [vp, vp]),
+    "tlc_kvcache8_create": (i32, [vp, i32, i32, i32, i32, i32, P(vp)]),
+    "tlc_kvcache8_destroy": (i32, [vp]),
+    "tlc_kvcache8_append": (i32, [vp, vp, i32, vp, vp, i32, i32, i32, vp]),
+    "tlc_kvcache8_rows": (i32, [vp, vp, i32, i32, i32, i32, i32, vp, vp]),
+    "tlc_attention8": (i32, [vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, vp, i32, f32]),
     "tlc_model_load_gguf": (i32, [vp, C.c_char_p, i32, i32, P(vp)]),
     "tlc_gguf_open": (i32, [C.c_char_p, P(vp)]),
     "tlc_gguf_close": (i32, [vp]),
@@ -142,6 +147,7 @@ PROTOTYPES = {
     "tlc_llama_set_sampling": (i32, [vp, f32, u64]),
     "tlc_sample_uniform_host": (f32, [u64, u32, u32]),
     "tlc_temperature_sample": (i32, [vp, vp, i32, i32, f32, P(f32), P(i32)]),
+    "tlc_token_logprobs": (i32, [vp, vp, i32, i32, vp, i32, vp, vp, vp, vp]),
     "tlc_weight_cache_open": (i32, [vp, C.c_char_p, i64, P(vp)]),
     "tlc_weight_cache_close": (i32, [vp]),
     "tlc_weight_cache_get": (i32, [vp, C.c_char_p, P(vp)]),

@@ -27,7 +27,8 @@ from . import _lib
 from ._lib import TensorError, check
 
 __all__ = ["Device", "Tensor", "QTensor", "TensorError", "linear", "rms_norm", "rope", "sigmoid", "mul", "add",
-           "silu", "swiglu", "softmax", "embedding", "norm_linear_multi", "swiglu_gate_up", "linear_residual"]
+           "silu", "swiglu", "softmax", "embedding", "norm_linear_multi", "swiglu_gate_up", "linear_residual",
+           "KVCache", "KVCache8", "token_logprobs"]
 
 
 class Device:
@@ -393,6 +394,39 @@ def temperature_sample(logits: Tensor, temperature: float = 1.0, uniforms=None) 
     return ids
 
 
+def token_logprobs(logits: Tensor, tokens=None, top_k: int = 0):
+    """How likely the model found ``tokens``, one for each row of ``logits`` [rows, vocab]: (log probabilities [rows],
+    entropies [rows], ids [rows, top_k], log probabilities [rows, top_k]) as host arrays.
+
+    The alternatives are the ``top_k`` (0 .. 32) largest logits, equal ones in the order of their ids.  A token of -1
+    has log probability 0 (padding).  Without ``tokens`` the first result is None.  Logits that are not finite carry
+    no probability, as in ``softmax``."""
+    vocab = logits.shape[-1]
+    rows, dev = logits.size // vocab, logits.dev
+    ids_t = None
+    if tokens is not None:
+        ids = np.ascontiguousarray(np.atleast_1d(tokens), dtype=np.int32).reshape(-1)
+        if ids.size != rows:
+            raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"token_logprobs: {ids.size} tokens for {rows} rows")
+        wrong = (ids < -1) | (ids >= vocab)
+        if wrong.any():
+            raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {ids[wrong][0]}, size {vocab}")
+        ids_t = _upload_i32(dev, ids)
+    if not 0 <= top_k <= 32:
+        raise TensorError(_lib.ERR_INVALID_OPERATION, f"token_logprobs: top_k {top_k} outside 0 .. 32")
+    per = 2 + 2 * top_k  # 4-byte words a row
+    out = Tensor(dev, (rows * per * 2,))
+    at = [out.ptr + 4 * rows * n for n in (0, 1, 2, 2 + top_k)]
+    check(dev.lib.tlc_token_logprobs(dev.handle, logits.ptr, rows, vocab, ids_t.ptr if ids_t is not None else None, top_k,
+                                     at[0] if ids_t is not None else None, at[1], at[2] if top_k else None,
+                                     at[3] if top_k else None))
+    host = np.empty(rows * per, np.float32)
+    if host.size:
+        check(dev.lib.tlc_download(dev.handle, host.ctypes.data, out.ptr, host.nbytes))
+    lp, entropy, ids, best = np.split(host, [rows, 2 * rows, (2 + top_k) * rows])
+    return (lp if ids_t is not None else None, entropy, ids.view(np.int32).reshape(rows, top_k), best.reshape(rows, top_k))
+
+
 def embedding(table: Tensor, ids) -> Tensor:
     if table.ndim != 2:
         raise TensorError(_lib.ERR_INVALID_OPERATION, "embedding table must be 2D [vocab, d]")
@@ -511,6 +545,110 @@ class KVCache:
         check(self.dev.lib.tlc_attention(self.dev.handle, self.handle, layer, q.ptr, out.ptr, batch, nq, n_heads,
                                          q_pos0, pos_t.ptr if pos_t is not None else None, max_keys, scale))
         return out
+
+
+class KVCache8:
+    """A KV cache in half the bytes of ``KVCache``: blocks of 64 positions of a KV head as 8-bit codes with one scale
+    (the block's largest magnitude / 127), the rows of a block that is not full yet in f16.
+
+    The same calls, and any sequence may be given a prompt (``sequence``).  Rows join at the end of a sequence or at
+    an earlier position (what lay behind it is gone).  The cache holds finite values: NaN becomes zero, an infinity
+    +-65504.  head_dim is 64 or 128; any number of query heads per KV head."""
+
+    def __init__(self, dev: Device, n_layers: int, n_kv_heads: int, head_dim: int, max_seq: int = 2048,
+                 max_batch: int = 1):
+        self.dev, self.handle = dev, None
+        self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
+        self.max_seq, self.max_batch = max_seq, max_batch
+        h = C.c_void_p()
+        check(dev.lib.tlc_kvcache8_create(dev.handle, n_layers, max_batch, max_seq, n_kv_heads, head_dim, C.byref(h)))
+        self.handle = h
+        self.lengths = np.zeros((n_layers, max_batch), np.int64)  # rows of each sequence, as the calls leave them
+
+    def __del__(self):
+        try:
+            if self.handle and self.dev.handle:
+                self.dev.lib.tlc_kvcache8_destroy(self.handle)
+            self.handle = None
+        except Exception:
+            pass
+
+    def append(self, layer: int, k: Tensor, v: Tensor, positions: Optional[np.ndarray] = None, sequence: int = 0,
+               position: Optional[int] = None) -> None:
+        """cache.append(layer, K, V): K/V are [m, n_kv_heads, head_dim] (or [m, n_kv_heads*head_dim]), m tokens of
+        ``sequence`` from ``position`` on (default: its end); with ``positions`` a token for each of the sequences
+        from ``sequence`` on, a negative position for none."""
+        row = self.n_kv_heads * self.head_dim
+        if k.size % row or k.size != v.size:
+            raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"KV rows must have {row} elements")
+        m = k.size // row
+        self._check(layer, sequence, 1 if positions is None else m)
+        held = self.lengths[layer, sequence:]
+        pos_t = None
+        if positions is None:
+            at = int(held[0]) if position is None else int(position)
+            if not 0 <= at <= held[0]:
+                raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {at}, size {held[0]}")
+        else:
+            at = 0
+            pos = np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
+            if pos.size != m:
+                raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"KV cache: {pos.size} positions for {m} rows")
+            wrong = (pos > held[:m]) | (pos >= self.max_seq)
+            if wrong.any():
+                raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {pos[wrong][0]}, size {held[:m][wrong][0]}")
+            pos_t = _upload_i32(self.dev, pos)
+        check(self.dev.lib.tlc_kvcache8_append(self.dev.handle, self.handle, layer, k.ptr, v.ptr, m, sequence, at,
+                                               pos_t.ptr if pos_t is not None else None))
+        if positions is None:
+            held[0] = at + m if m else held[0]
+        else:
+            held[:m] = np.where(pos >= 0, pos + 1, held[:m])
+
+    def layer_arrays(self, layer: int, batch_index: int = 0, length: Optional[int] = None):
+        """get_k / get_v: host copies [len, n_kv_heads, head_dim] of the values the cache stands for."""
+        self._check(layer, batch_index, 1)
+        n = int(self.lengths[layer, batch_index]) if length is None else length
+        out = [self.dev.empty((n, self.n_kv_heads, self.head_dim)) for _ in range(2)]
+        check(self.dev.lib.tlc_kvcache8_rows(self.dev.handle, self.handle, layer, batch_index, 1, 0, n, out[0].ptr,
+                                             out[1].ptr))
+        return [t.numpy() for t in out]
+
+    def attention(self, layer: int, q: Tensor, n_heads: int, q_pos0: int = 0, batch: int = 1,
+                  positions: Optional[np.ndarray] = None, scale: Optional[float] = None, sequence: int = 0) -> Tensor:
+        """softmax(q.K^T * scale + causal mask).V for q [batch*n_queries, n_heads, head_dim] of the sequences from
+        ``sequence`` on; a negative position marks an idle slot, whose output rows are zeros."""
+        D = self.head_dim
+        if n_heads < 1 or batch < 1 or q.size % (n_heads * D * batch):
+            raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"attention: q has {q.size} elements")
+        self._check(layer, sequence, batch)
+        nq = q.size // (n_heads * D * batch)
+        held = self.lengths[layer, sequence:sequence + batch]
+        pos_t, max_keys = None, q_pos0 + nq
+        if positions is None:
+            wrong = held < q_pos0 + nq
+            if wrong.any():
+                raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {q_pos0 + nq - 1}, size {held[wrong][0]}")
+        else:
+            pos = np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
+            if pos.size != batch:
+                raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"attention: {pos.size} positions for {batch} sequences")
+            if (pos >= held).any():
+                raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {pos[pos >= held][0]}, size {held[pos >= held][0]}")
+            pos_t = _upload_i32(self.dev, pos)
+            max_keys = max(int(pos.max()) + 1, 1)
+        out = Tensor._new(self.dev, q.shape, q.size)
+        scale = 1.0 / math.sqrt(D) if scale is None else scale
+        check(self.dev.lib.tlc_attention8(self.dev.handle, self.handle, layer, q.ptr, out.ptr, batch, nq, n_heads, sequence,
+                                          q_pos0, pos_t.ptr if pos_t is not None else None, max_keys, scale))
+        return out
+
+    def _check(self, layer: int, sequence: int, count: int) -> None:
+        if not 0 <= layer < self.n_layers:
+            raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {layer}, size {self.n_layers}")
+        if sequence < 0 or sequence + count > self.max_batch:
+            raise TensorError(_lib.ERR_SHAPE_MISMATCH,
+                              f"KV cache: sequences {sequence} .. {sequence + count - 1} exceed its {self.max_batch}")
 
 
 def linear_residual(x: Tensor, weight: QTensor, residual: Tensor) -> Tensor:

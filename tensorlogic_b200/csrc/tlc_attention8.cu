@@ -1,0 +1,460 @@
+// Grouped-query attention over the 8-bit KV cache (tlc_kv8.h).
+//
+//   o_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp(scale q_r.k_j - m_r),   j = 0 .. position of row r
+//
+// On sealed blocks k_j = s_k c_j and v_j = s_v c_j with integer codes c and one scale per block, so the tensor cores
+// multiply the codes as they are (exact in f16) and s_k multiplies a score, s_v a block's product.
+//
+// attention8_kernel: a CTA of four warps owns 8 * NT (query, head) rows that share a KV head, queries in the order
+// (position, head of the group), and every nsplit-th quad of blocks; a warp takes one block at a time, alone:
+//   S^T = K.Q^T  16 keys x 8 rows a product, codes as the 16-row operand (PRMT makes it, tlc_kv8.h)
+//   P            f32 maximum and sums over the keys of a row, P rounded to f16, times 2^12 so that small
+//                probabilities keep their bits; the sum is of the rounded values
+//   O^T += V^T.P P turned over by movmatrix, f32 accumulators of the block, scaled by s_v when they join O
+// A warp's blocks arrive by cp.async in a ring of its own; a lane copies the very bytes it will use, so a warp needs no
+// barrier and no other lane until the CTA's four results are merged in shared memory.  Where keys are shared out over
+// CTAs they leave (maximum, sum, O) in the cache's workspace and the last one (a ticket) merges.
+#include <cuda_fp16.h>
+
+#include "tlc_kv8.h"
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr float kShift = 12.f;        // P is held times 2^12
+constexpr float kUp = 16777216.f;     // the codes' 2^24
+constexpr float kLog2e = 1.4426950408889634f;
+template <int D> constexpr int stages() { return D == 128 ? 3 : 6; }  // of 64 * D bytes (K or V of a block) per warp
+
+struct Params {
+    const __half *q;  // [batch * I, H, D]
+    __half *out;
+    Kv8View c;
+    int I, H, G;
+    int pos0;              // position of query 0 (positions == null)
+    const int *positions;  // device int32[batch]: position of each sequence's query; negative: none
+    int key_limit;         // keys the launch was sized for
+    float scale;
+    int row_tiles, nsplit;
+    float *partial;  // [CTA][row][2], then [CTA][row][D]
+    int *tickets;
+    tlc_dev_status *status;
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t low2(uint32_t w) { return __byte_perm(w, 0, 0x4140); }
+__device__ __forceinline__ uint32_t high2(uint32_t w) { return __byte_perm(w, 0, 0x4342); }
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
+    constexpr int ROWS = 8 * NT, STAGE = kKv8Block * D, ST = stages<D>(), LOADS = STAGE / 512, PITCH = D + 4;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
+    __shared__ int sm_last;
+    tlc_pdl_after_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, hk = blockIdx.y, b = blockIdx.z;
+    const int rows = p.I * p.G, r0 = rt * ROWS;
+    const size_t head = (size_t)b * p.c.n_kv_heads + hk;
+    auto row_of = [&](int r) { return ((size_t)b * p.I + r / p.G) * p.H + hk * p.G + r % p.G; };
+
+    const int at0 = p.positions ? p.positions[b] : p.pos0, held = p.c.lengths[head * 2];
+    const int keys = min(held, p.key_limit);  // what a row may see at most
+    if (at0 >= 0 && at0 > keys - p.I && tid == 0 && split == 0 && atomicCAS(&p.status->code, 0, TLC_DEV_INDEX) == 0)
+        p.status->where = 400 + b;  // a query in front of its key: it sees what there is, and that is said
+    const int pos0 = min(at0, keys);
+    const int last = min(rows, r0 + ROWS) - 1;  // last row of the tile
+    const int seen = pos0 < 0 ? 0 : min(keys, pos0 + last / p.G + 1);
+    if (seen <= 0) {  // an idle slot, or nothing in the cache
+        if (split == 0)
+            for (int i = tid; i < (last - r0 + 1) * (D / 8); i += kThreads)
+                *reinterpret_cast<uint4 *>(p.out + row_of(r0 + i / (D / 8)) * D + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const int units = (seen + kKv8Block - 1) / kKv8Block, sealed = held / kKv8Block;
+    const int stride = p.nsplit * kWarps, u0 = split * kWarps + warp;
+    const uint8_t *codes = p.c.codes + head * p.c.n_blocks * (2 * STAGE);
+    const float *scales = p.c.scales + head * p.c.n_blocks * 2;
+
+    // The ring: K and V of a block in turn.
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)(warp * ST * STAGE + lane * 16);
+    const int n_sealed = min(units, sealed), items = u0 < n_sealed ? 2 * ((n_sealed - u0 + stride - 1) / stride) : 0;
+    auto fetch = [&](int item) {
+        if (item < items) {
+            const uint8_t *src = codes + ((size_t)(u0 + (item >> 1) * stride) * 2 + (item & 1)) * STAGE + lane * 16;
+            const uint32_t dst = ring + (uint32_t)(item % ST * STAGE);
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) copy16(dst + i * 512, src + i * 512);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");  // (empty ones keep the count)
+    };
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++) fetch(i);
+
+    // Queries: row r0 + 8 nt + g as the 8-column operand, and -128 sum q for rows 2t and 2t + 1
+    uint32_t qf[NT][D / 16][2];
+    float start[NT][2];
+    int end[NT][2];  // keys that rows 2t and 2t + 1 see
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = r0 + 8 * nt + g;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < rows) v = *reinterpret_cast<const uint4 *>(p.q + row_of(r) * D + c * 32 + t * 8);
+            qf[nt][2 * c][0] = v.x;
+            qf[nt][2 * c][1] = v.y;
+            qf[nt][2 * c + 1][0] = v.z;
+            qf[nt][2 * c + 1][1] = v.w;
+            const __half2 *h = reinterpret_cast<const __half2 *>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum += __low2float(h[e]) + __high2float(h[e]);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            start[nt][e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * (-128.f / kUp);
+            end[nt][e] = min(keys, pos0 + min(r0 + 8 * nt + 2 * t + e, rows - 1) / p.G + 1);
+        }
+    }
+    const int all_see = min(keys, pos0 + r0 / p.G + 1);  // keys that every row sees
+
+    float m_run[NT][2], l_run[NT][2], o[NT][D / 16][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m_run[nt][0] = m_run[nt][1] = -INFINITY;
+        l_run[nt][0] = l_run[nt][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    }
+
+    // Softmax of a block's scores s[kg][nt][..] (keys 16 kg + kv8_key(g), .. + kv8_key(g + 8) of rows 2t, 2t + 1): P as
+    // the second product's operand, its sums, and what the rows' O has to be multiplied with.
+    auto softmax = [&](int u, float (&s)[4][NT][4], float factor, uint32_t (&pf)[4][NT][2], float (&psum)[NT][2], float (&corr)[NT][2]) {
+        const bool masked = (u + 1) * kKv8Block > all_see;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float x = s[kg][nt][e] * factor;
+                    if (masked && u * kKv8Block + 16 * kg + 4 * (g >> 1) + (g & 1) + 2 * (e >> 1) >= end[nt][e & 1]) x = -INFINITY;
+                    s[kg][nt][e] = x;
+                    mx[e & 1] = fmaxf(mx[e & 1], x);
+                }
+            float shift[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
+                const float m_new = fmaxf(m_run[nt][e], mx[e]), m_safe = m_new == -INFINITY ? 0.f : m_new;
+                corr[nt][e] = exp2_of(m_run[nt][e] - m_safe);
+                m_run[nt][e] = m_new;
+                shift[e] = kShift - m_safe;
+                psum[nt][e] = 0.f;
+            }
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const __half2 v = __floats2half2_rn(exp2_of(s[kg][nt][2 * h] + shift[0]), exp2_of(s[kg][nt][2 * h + 1] + shift[1]));
+                    psum[nt][0] += __low2float(v);
+                    psum[nt][1] += __high2float(v);
+                    pf[kg][nt][h] = turned(*reinterpret_cast<const uint32_t *>(&v));
+                }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) psum[nt][e] += __shfl_xor_sync(0xffffffffu, psum[nt][e], d);
+                l_run[nt][e] = l_run[nt][e] * corr[nt][e] + psum[nt][e];
+            }
+        }
+    };
+    // O of 16 values of d (index dt): times corr, plus the block's product
+    auto join = [&](int dt, int nt, const float (&acc)[4], float factor, const float (&corr)[NT][2]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[nt][dt][e] = o[nt][dt][e] * corr[nt][e & 1] + acc[e] * factor;
+    };
+
+    int item = 0;
+    for (int u = u0; u < n_sealed; u += stride) {
+        const float sk = scales[2 * u], sv = scales[2 * u + 1];
+        float s[4][NT][4], psum[NT][2], corr[NT][2];
+        uint32_t pf[4][NT][2];
+        fetch(item + ST - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        uint32_t at = ring + (uint32_t)(item % ST * STAGE);
+#pragma unroll
+        for (int kg = 0; kg < 4; kg++) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                s[kg][nt][0] = s[kg][nt][2] = start[nt][0];
+                s[kg][nt][1] = s[kg][nt][3] = start[nt][1];
+            }
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                const uint4 w = lds128(at + (uint32_t)((kg * (D / 32) + c) * 512));
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    mma(s[kg][nt], low2(w.x), low2(w.z), high2(w.x), high2(w.z), qf[nt][2 * c][0], qf[nt][2 * c][1]);
+                    mma(s[kg][nt], low2(w.y), low2(w.w), high2(w.y), high2(w.w), qf[nt][2 * c + 1][0], qf[nt][2 * c + 1][1]);
+                }
+            }
+        }
+        item++;
+        softmax(u, s, kUp * sk * p.scale * kLog2e, pf, psum, corr);
+        fetch(item + ST - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        at = ring + (uint32_t)(item % ST * STAGE);
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) {
+            float acc[2][NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[0][nt][e] = acc[1][nt][e] = psum[nt][e & 1] * (-128.f / kUp);
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++) {
+                const uint4 w = lds128(at + (uint32_t)((kg * (D / 32) + c) * 512));
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    mma(acc[0][nt], low2(w.x), low2(w.y), high2(w.x), high2(w.y), pf[kg][nt][0], pf[kg][nt][1]);
+                    mma(acc[1][nt], low2(w.z), low2(w.w), high2(w.z), high2(w.w), pf[kg][nt][0], pf[kg][nt][1]);
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                join(2 * c, nt, acc[0][nt], kUp * sv, corr);
+                join(2 * c + 1, nt, acc[1][nt], kUp * sv, corr);
+            }
+        }
+        item++;
+    }
+    // The open block, where this warp's turn has come to it: f16 rows straight from memory.
+    if (units > sealed && sealed % stride == u0) {
+        const uint4 *kt = reinterpret_cast<const uint4 *>(p.c.open + head * (2 * STAGE)) + lane, *vt = kt + STAGE / 8;
+        float s[4][NT][4], psum[NT][2], corr[NT][2];
+        uint32_t pf[4][NT][2];
+#pragma unroll
+        for (int kg = 0; kg < 4; kg++) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) s[kg][nt][0] = s[kg][nt][1] = s[kg][nt][2] = s[kg][nt][3] = 0.f;
+#pragma unroll
+            for (int k16 = 0; k16 < D / 16; k16++) {
+                const uint4 w = kt[(kg * (D / 16) + k16) * 32];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma(s[kg][nt], w.x, w.z, w.y, w.w, qf[nt][k16][0], qf[nt][k16][1]);
+            }
+        }
+        softmax(sealed, s, p.scale * kLog2e, pf, psum, corr);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; dt++) {
+            float acc[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++) {
+                const uint4 w = vt[(kg * (D / 16) + dt) * 32];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma(acc[nt], w.x, w.z, w.y, w.w, pf[kg][nt][0], pf[kg][nt][1]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) join(dt, nt, acc[nt], 1.f, corr);
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the ring's place takes the four warps' O: [warp][row][D], rows PITCH apart
+
+    float *so = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        if (g == 0) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                sm_m[warp][8 * nt + 2 * t + e] = m_run[nt][e];
+                sm_l[warp][8 * nt + 2 * t + e] = l_run[nt][e];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) so[(warp * ROWS + 8 * nt + 2 * t + (e & 1)) * PITCH + 16 * i + g + 8 * (e >> 1)] = o[nt][i][e];
+    }
+    __syncthreads();
+
+    // 16 threads a row, PER values each
+    constexpr int PER = D / 16;
+    const size_t slot = (((size_t)b * p.c.n_kv_heads + hk) * p.row_tiles + rt) * p.nsplit;
+    float *part_ml = p.partial, *part_o = p.partial + (size_t)kKv8MaxCtas * kKv8MaxRows * 2;
+    auto store = [&](int r, int d0, const float (&acc)[PER], float l) {
+        if (r0 + r >= rows) return;
+        const float inv = 1.0f / l;  // (the largest p is 2^12; a row whose scores are NaN stays NaN)
+        __align__(16) __half h[PER];
+#pragma unroll
+        for (int i = 0; i < PER; i++) h[i] = __float2half_rn(acc[i] * inv);
+        __half *to = p.out + row_of(r0 + r) * D + d0;
+        if constexpr (PER == 8) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(h);
+        else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(h);
+    };
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = 8 * nt + (tid >> 4), d0 = (tid & 15) * PER;
+        float M = -INFINITY, L = 0.f, acc[PER];
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) M = fmaxf(M, sm_m[w][r]);
+#pragma unroll
+        for (int i = 0; i < PER; i++) acc[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const float wgt = sm_m[w][r] == -INFINITY && sm_l[w][r] == 0.f ? 0.f : exp2_of(sm_m[w][r] - (M == -INFINITY ? 0.f : M));
+            L += sm_l[w][r] * wgt;
+#pragma unroll
+            for (int i = 0; i < PER; i++) acc[i] += so[(w * ROWS + r) * PITCH + d0 + i] * wgt;
+        }
+        if (p.nsplit == 1) {
+            store(r, d0, acc, L);
+            continue;
+        }
+        const size_t at = (slot + split) * ROWS + r;
+        if ((tid & 15) == 0) *reinterpret_cast<float2 *>(part_ml + at * 2) = make_float2(M, L);
+#pragma unroll
+        for (int i = 0; i < PER; i += 4)
+            *reinterpret_cast<float4 *>(part_o + at * D + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+    }
+    if (p.nsplit == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+        int *ticket = p.tickets + slot / p.nsplit;
+        sm_last = atomicAdd(ticket, 1) == p.nsplit - 1;
+        if (sm_last) *ticket = 0;
+    }
+    __syncthreads();
+    if (!sm_last) return;
+    __threadfence();
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = 8 * nt + (tid >> 4), d0 = (tid & 15) * PER;
+        const size_t at = slot * ROWS + r;
+        float M = -INFINITY, L = 0.f, acc[PER];
+#pragma unroll 8
+        for (int sp = 0; sp < p.nsplit; sp++) M = fmaxf(M, __ldcg(part_ml + (at + (size_t)sp * ROWS) * 2));
+#pragma unroll
+        for (int i = 0; i < PER; i++) acc[i] = 0.f;
+#pragma unroll 4
+        for (int sp = 0; sp < p.nsplit; sp++) {
+            const size_t a = at + (size_t)sp * ROWS;
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_ml + a * 2));
+            const float wgt = ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2_of(ml.x - (M == -INFINITY ? 0.f : M));
+            L += ml.y * wgt;
+#pragma unroll
+            for (int i = 0; i < PER; i += 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_o + a * D + d0 + i));
+                acc[i] += v.x * wgt;
+                acc[i + 1] += v.y * wgt;
+                acc[i + 2] += v.z * wgt;
+                acc[i + 3] += v.w * wgt;
+            }
+        }
+        store(r, d0, acc, L);
+    }
+}
+
+template <int D, int NT>
+int32_t launch(tlc_ctx *ctx, const Params &p, dim3 grid) {
+    constexpr size_t ring = (size_t)kWarps * stages<D>() * kKv8Block * D, merge = (size_t)kWarps * 8 * NT * (D + 4) * sizeof(float);
+    constexpr size_t smem = ring > merge ? ring : merge;
+    static bool configured[64] = {};
+    if (!configured[ctx->device & 63]) {
+        TLC_CUDA(cudaFuncSetAttribute(attention8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        TLC_CUDA(cudaFuncSetAttribute(attention8_kernel<D, NT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                      cudaSharedmemCarveoutMaxShared));
+        configured[ctx->device & 63] = true;
+    }
+    const cudaError_t le = tlc_launch_pdl(ctx, attention8_kernel<D, NT>, grid, dim3(kThreads), smem, p);
+    if (le != cudaSuccess) {
+        cudaGetLastError();
+        return tlc_fail(TLC_ERR_CUDA, "attention8 launch failed: %s", cudaGetErrorString(le));
+    }
+    TLC_CHECK_LAUNCH(ctx);
+    return TLC_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t layer, const void *q_dev, void *out_dev,
+                                  int32_t batch, int32_t n_queries, int32_t n_heads, int32_t sequence, int32_t q_pos0,
+                                  const int32_t *positions_dev, int32_t max_keys, float scale) {
+    if (int32_t rc = tlc_enter(ctx)) return rc;
+    tlc_perf_scope perf(ctx, "attention8(batch=%d, queries=%d, heads=%d)", batch, n_queries, n_heads);
+    TLC_REQUIRE(q_dev && out_dev, TLC_ERR_INVALID_OPERATION, "attention8: null pointer");
+    TLC_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) == 0, TLC_ERR_INVALID_OPERATION,
+                "attention8: queries and output must be 16-byte aligned");
+    TLC_REQUIRE(batch >= 1, TLC_ERR_SHAPE_MISMATCH, "attention8: batch %d", batch);
+    if (int32_t rc = kv8_check(ctx, cache, "attention8", layer, sequence, batch)) return rc;
+    const int D = cache->head_dim, Hkv = cache->n_kv_heads;
+    TLC_REQUIRE(n_heads >= 1 && n_heads % Hkv == 0, TLC_ERR_SHAPE_MISMATCH, "attention8: %d query heads over %d KV heads",
+                n_heads, Hkv);
+    TLC_REQUIRE(n_queries >= 1 && (!positions_dev || n_queries == 1), TLC_ERR_INVALID_OPERATION,
+                "attention8: per-sequence positions need one query per sequence");
+    TLC_REQUIRE(positions_dev || (q_pos0 >= 0 && q_pos0 <= cache->max_seq), TLC_ERR_INDEX,
+                "Index out of bounds: index %d, size %d", q_pos0, cache->max_seq);
+    const long long T = positions_dev ? max_keys : (long long)q_pos0 + n_queries;
+    TLC_REQUIRE(T >= 1 && T <= cache->max_seq, TLC_ERR_INDEX, "Index out of bounds: index %lld, size %d", T, cache->max_seq);
+    const int G = n_heads / Hkv;
+    TLC_REQUIRE(batch <= 65535 && (long long)n_queries * G <= INT_MAX / 64, TLC_ERR_INVALID_DIMENSION,
+                "attention8: %d sequences of %d queries", batch, n_queries);
+    Params p{};
+    p.q = static_cast<const __half *>(q_dev);
+    p.out = static_cast<__half *>(out_dev);
+    p.c = kv8_view(cache, layer, sequence);
+    p.I = n_queries;
+    p.H = n_heads;
+    p.G = G;
+    p.pos0 = q_pos0;
+    p.positions = positions_dev;
+    p.key_limit = (int)T;
+    p.scale = scale;
+    p.partial = cache->partial;
+    p.tickets = cache->tickets;
+    p.status = ctx->dev_status;
+    const int nt = n_queries * G > 8 ? 2 : 1;
+    p.row_tiles = (n_queries * G + 8 * nt - 1) / (8 * nt);
+    // Keys are shared out until there are two CTAs an SM, and no further than a block a warp.
+    const long long groups = (long long)batch * Hkv * p.row_tiles, units = (T + kKv8Block - 1) / kKv8Block;
+    long long nsplit = (2 * ctx->sm_count + groups - 1) / groups;
+    if (nsplit > (units + kWarps - 1) / kWarps) nsplit = (units + kWarps - 1) / kWarps;
+    if (nsplit < 1 || groups > kKv8Tickets) nsplit = 1;
+    while (nsplit > 1 && groups * nsplit > kKv8MaxCtas) nsplit--;
+    p.nsplit = (int)nsplit;
+    const dim3 grid((unsigned)(p.row_tiles * nsplit), (unsigned)Hkv, (unsigned)batch);
+    if (D == 64) return nt == 1 ? launch<64, 1>(ctx, p, grid) : launch<64, 2>(ctx, p, grid);
+    return nt == 1 ? launch<128, 1>(ctx, p, grid) : launch<128, 2>(ctx, p, grid);
+}

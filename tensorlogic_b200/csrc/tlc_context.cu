@@ -275,6 +275,8 @@ int32_t tlc_status_after_sync(tlc_ctx *ctx) {
         if (code < TLC_DEV_INDEX)  // a kernel that gave up may have left a hand-over flag behind
             cudaMemsetAsync(ctx->wt_flags, 0, (size_t)ctx->sm_count * sizeof(int), ctx->stream);
         cudaStreamSynchronize(ctx->stream);
+        if (code == TLC_DEV_INDEX && where == TLC_WHERE_TOKEN)
+            return tlc_fail(TLC_ERR_INDEX, "Index out of bounds: a target token lies outside the vocabulary");
         if (code == TLC_DEV_INDEX)
             return tlc_fail(TLC_ERR_INDEX, "Index out of bounds: a sequence position lies outside the KV cache "
                             "(site %d); the access was skipped", where);

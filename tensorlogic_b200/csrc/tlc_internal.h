@@ -24,6 +24,8 @@ struct tlc_dev_status {
 // TLC_DEV_INDEX means a kernel met a sequence position outside its cache and skipped the
 // access (TLC_ERR_INDEX).
 #define TLC_DEV_INDEX 16
+// `where` of a target token outside the vocabulary (other sites are numbers below it).
+#define TLC_WHERE_TOKEN (1 << 30)
 
 struct tlc_pool {
     // idle buffers by class size

@@ -1,0 +1,351 @@
+// Log probabilities of given tokens, entropy and the likeliest alternatives of logit rows, in one pass.
+//
+//   S = sum exp(x - m),  log p(t) = x_t - m - ln S,  H = ln S - sum exp(x - m) (x - m) / S,  m = max x (finite x only)
+//
+// A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary that its 512 threads hold in registers
+// (64 values a thread): read once, then the maximum, then the exponentials.  x log2(e) + c with c = -m log2(e) is one
+// fused multiply-add; c is off by some delta, which multiplies all exponentials alike and is divided out at the end,
+// so that large logits lose nothing.
+//
+// Alternatives: (value, lowest id first) is one 48-bit key per logit, so no two are equal.  The k-th largest of the best
+// keys of 128 groups of four threads is a bound that at least k logits reach, and none but those of at most k groups
+// can: these few are collected and ranked by counting.
+#include <cuda_fp16.h>
+
+#include "tlc_internal.h"
+
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32, kPieces = 8;  // 16-byte pieces a thread
+constexpr int kSlice = kThreads * kPieces * 8;                      // values a CTA holds at a time
+constexpr int kMaxTop = 32, kGroups = kThreads / 4;
+constexpr int kList = kMaxTop * kPieces * 8 * 4 + kMaxTop;  // what k groups hold, and the best of earlier slices
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMaxCluster = 8;
+
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct LogprobParams {
+    const __half *logits;
+    const int *targets;
+    float *logprobs, *entropy, *top_logprobs;
+    int *top_ids;
+    int rows, vocab, top, cluster;
+    tlc_dev_status *status;
+};
+struct Sums {
+    float m, s, t;  // maximum, sum of e^(x - m), sum of e^(x - m) (x - m) log2(e)
+};
+// Those of two disjoint sets.
+__device__ __forceinline__ Sums joined(const Sums &a, const Sums &b) {
+    const float m = fmaxf(a.m, b.m);
+    if (m == -INFINITY) return a;
+    const float da = fmaxf((a.m - m) * kLog2e, -1e30f), db = fmaxf((b.m - m) * kLog2e, -1e30f);  // (an empty set's is -inf)
+    const float wa = exp2_of(da), wb = exp2_of(db);
+    return {m, wa * a.s + wb * b.s, wa * (a.t + da * a.s) + wb * (b.t + db * b.s)};
+}
+
+// Larger for a larger value, then for a smaller id; 0: no logit.
+__device__ __forceinline__ unsigned long long key_of(__half x, unsigned id) {
+    const unsigned short b = __half_as_ushort(x);
+    const unsigned v = (b & 0x8000) ? (unsigned short)~b : (unsigned short)(b | 0x8000);
+    return (unsigned long long)v << 32 | (0xFFFFFFFFu - id);
+}
+__device__ __forceinline__ __half value_of(unsigned long long key) {
+    const unsigned short v = (unsigned short)(key >> 32);
+    return __ushort_as_half((v & 0x8000) ? (unsigned short)(v & 0x7FFF) : (unsigned short)~v);
+}
+
+template <bool TOP>
+__global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParams p) {
+    extern __shared__ __align__(16) unsigned long long list[];  // [kList] (TOP)
+    __shared__ __align__(16) unsigned long long group_best[kGroups];
+    __shared__ unsigned long long best[kMaxCluster][kMaxTop];  // of this CTA's slices; in the first CTA, of all
+    __shared__ Sums sums[kMaxCluster];
+    __shared__ float warp_max[kWarps], warp_s[kWarps], warp_t[kWarps];
+    __shared__ unsigned long long bound;
+    __shared__ int n_list;
+    if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    tlc_pdl_after_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blockIdx.x % p.cluster, row = blockIdx.x / p.cluster;
+    const __half *x0 = p.logits + (size_t)row * p.vocab;
+    // The row in 16-byte pieces of memory: the first and the last may reach into other rows, and past the array.
+    const int ahead = (int)(((uintptr_t)x0 & 15) >> 1);  // values of the first piece in front of the row
+    const __half *base = x0 - ahead, *lo = p.logits, *hi = p.logits + (size_t)p.rows * p.vocab;
+    const long long pieces = ((long long)ahead + p.vocab + 7) / 8, share = (pieces + p.cluster - 1) / p.cluster;
+    const long long first = rank * share, end = first + share < pieces ? first + share : pieces;
+
+    if (TOP && tid < p.top) best[0][tid] = 0;
+    Sums run = {-INFINITY, 0.f, 0.f};
+    const __half2 neg_inf = __float2half2_rn(-INFINITY), neg_zero = __floats2half2_rn(-0.f, -0.f);
+    for (long long p0 = first; p0 < end; p0 += kThreads * kPieces) {
+        __half2 v[kPieces * 4];
+#pragma unroll
+        for (int i = 0; i < kPieces; i++) {
+            const long long at = p0 + tid + i * kThreads;
+            const __half *src = base + at * 8;
+            uint4 w = make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);  // -inf
+            if (at < end) {
+                if (src >= lo && src + 8 <= hi) {
+                    w = *reinterpret_cast<const uint4 *>(src);
+                } else {
+                    __half *h = reinterpret_cast<__half *>(&w);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (src + e >= lo && src + e < hi) h[e] = src[e];
+                }
+                if (at == 0 || at + 1 == pieces) {  // not this row's
+                    unsigned short *h = reinterpret_cast<unsigned short *>(&w);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (at * 8 + e < ahead || at * 8 + e >= (long long)ahead + p.vocab) h[e] = 0xFC00;
+                }
+            }
+            const __half2 *h = reinterpret_cast<const __half2 *>(&w);
+            // x * -0 + x is NaN for what is not finite, x for the rest (+0 for -0); the maximum passes over NaN
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * i + e] = __hmax2(__hfma2(h[e], neg_zero, h[e]), neg_inf);
+        }
+        __half2 mx = v[0];
+#pragma unroll
+        for (int e = 1; e < kPieces * 4; e++) mx = __hmax2(mx, v[e]);
+        const float mine = fmaxf(__low2float(mx), __high2float(mx));
+        float m = mine;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        __syncthreads();  // (what the slice before left here has been read)
+        if (lane == 0) warp_max[warp] = m;
+        if (TOP) {
+            // this group's best key: of the values equal to a thread's maximum, the first
+            unsigned long long k = 0;
+            if (mine > -INFINITY) {
+                const __half want = __float2half_rn(mine);
+                unsigned id = 0;
+#pragma unroll
+                for (int e = kPieces * 4 - 1; e >= 0; e--) {
+                    const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kThreads) * 8 + 2 * (e & 3) - ahead);
+                    if (__heq(__high2half(v[e]), want)) id = at + 1;
+                    if (__heq(__low2half(v[e]), want)) id = at;
+                }
+                k = key_of(want, id);
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o *= 2) {
+                const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
+                k = other > k ? other : k;
+            }
+            if ((tid & 3) == 0) group_best[tid >> 2] = k;
+            if (tid == 0) {
+                bound = 0;
+                n_list = p.top;
+            }
+        }
+        __syncthreads();
+        m = warp_max[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; w++) m = fmaxf(m, warp_max[w]);
+        if (TOP) {
+            // group tid / 4, against a quarter of the others: the one with k - 1 better ones is the bound
+            const unsigned long long own = group_best[tid >> 2];
+            int better = 0;
+#pragma unroll 8
+            for (int i = 0; i < kGroups / 4; i++) better += group_best[4 * i + (tid & 3)] > own;
+            better += __shfl_xor_sync(0xffffffffu, better, 1);
+            better += __shfl_xor_sync(0xffffffffu, better, 2);
+            if ((tid & 3) == 0 && better == p.top - 1 && own > 0) bound = own;
+            if (tid < p.top) list[tid] = best[0][tid];
+        }
+        float s = 0.f, t = 0.f, delta = 0.f;
+        if (m > -INFINITY) {
+            const float c = -(m * kLog2e);
+            delta = fmaf(m, kLog2e, c);
+            float s4[4] = {0.f, 0.f, 0.f, 0.f}, t4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < kPieces * 4; e++) {
+                const float2 f = __half22float2(v[e]);
+                // (2^-200 is zero; e t of a logit of -inf would be NaN)
+                const float a = fmaxf(fmaf(f.x, kLog2e, c), -200.f), b = fmaxf(fmaf(f.y, kLog2e, c), -200.f);
+                const float ea = exp2_of(a), eb = exp2_of(b);
+                s4[2 * (e & 1)] += ea;
+                s4[2 * (e & 1) + 1] += eb;
+                t4[2 * (e & 1)] = fmaf(ea, a, t4[2 * (e & 1)]);
+                t4[2 * (e & 1) + 1] = fmaf(eb, b, t4[2 * (e & 1) + 1]);
+            }
+            s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            t = (t4[0] + t4[1]) + (t4[2] + t4[3]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            t += __shfl_xor_sync(0xffffffffu, t, o);
+        }
+        if (lane == 0) {
+            warp_s[warp] = s;
+            warp_t[warp] = t;
+        }
+        __syncthreads();
+        if (TOP) {
+            const unsigned long long least = bound;  // 0: fewer than k groups have anything
+            // (a thread whose maximum is below the bound's value has nothing to add)
+            if (mine > -INFINITY && (least == 0 || mine >= __half2float(value_of(least)))) {
+#pragma unroll
+                for (int e = 0; e < kPieces * 4; e++) {
+                    const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kThreads) * 8 + 2 * (e & 3) - ahead);
+                    const __half a = __low2half(v[e]), b = __high2half(v[e]);
+                    if (__hgt(a, __low2half(neg_inf)) && key_of(a, at) >= least) list[atomicAdd(&n_list, 1)] = key_of(a, at);
+                    if (__hgt(b, __low2half(neg_inf)) && key_of(b, at + 1) >= least) list[atomicAdd(&n_list, 1)] = key_of(b, at + 1);
+                }
+            }
+        }
+        s = t = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            s += warp_s[w];
+            t += warp_t[w];
+        }
+        const float back = exp2_of(-delta);
+        run = joined(run, {m, s * back, (t - delta * s) * back});
+        if (TOP) {
+            __syncthreads();
+            const int n = n_list;
+            if (tid < p.top) best[0][tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += kThreads) {
+                const unsigned long long own = list[i];
+                int rank_of = 0;
+                for (int j = 0; j < n; j++) rank_of += list[j] > own;
+                if (own > 0 && rank_of < p.top) best[0][rank_of] = own;
+            }
+        }
+    }
+    // The first CTA of the row joins what the others found.
+    if (p.cluster > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the row runs
+        __syncthreads();
+        auto remote = [&](const void *at) {
+            uint32_t a;
+            asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)));
+            return a;
+        };
+        if (rank > 0) {
+            if (TOP && tid < p.top)
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&best[rank][tid])), "l"(best[0][tid]) : "memory");
+            if (tid < 3)
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(&sums[rank].m) + 4 * tid), "f"(tid == 0 ? run.m : tid == 1 ? run.s : run.t)
+                             : "memory");
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank > 0) return;
+        for (int i = 1; i < p.cluster; i++) run = joined(run, sums[i]);
+    } else {
+        __syncthreads();
+    }
+    const bool any = run.m > -INFINITY;
+    const float ln_s = any ? logf(run.s) : 0.f;
+    if (tid == 0) {
+        if (p.logprobs) {
+            const int target = p.targets[row];
+            float lp = 0.f;
+            if (target >= 0 && target < p.vocab) {
+                const float x = __half2float(x0[target]);
+                lp = isfinite(x) ? (x - run.m) - ln_s : -INFINITY;
+            } else if (target != -1) {
+                lp = __int_as_float(0x7FC00000);
+                if (atomicCAS(&p.status->code, 0, TLC_DEV_INDEX) == 0) p.status->where = TLC_WHERE_TOKEN;
+            }
+            p.logprobs[row] = lp;
+        }
+        if (p.entropy) p.entropy[row] = any ? fmaxf(ln_s - kLn2 * run.t / run.s, 0.f) : 0.f;
+    }
+    if (!TOP) return;
+    // Rank of each CTA's best among all of them
+    const int n = p.cluster * p.top;
+    if (tid < n) {
+        const unsigned long long own = best[tid / p.top][tid % p.top];
+        int rank_of = 0, there = 0;
+        for (int c = 0; c < p.cluster; c++)
+            for (int j = 0; j < p.top; j++) {
+                rank_of += best[c][j] > own;
+                there += best[c][j] > 0;
+            }
+        const size_t out = (size_t)row * p.top;
+        if (own > 0 && rank_of < p.top) {
+            p.top_ids[out + rank_of] = (int)(0xFFFFFFFFu - (unsigned)own);
+            p.top_logprobs[out + rank_of] = (__half2float(value_of(own)) - run.m) - ln_s;
+        }
+        if (tid < p.top && tid >= there) {
+            p.top_ids[out + tid] = -1;
+            p.top_logprobs[out + tid] = -INFINITY;
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int32_t rows, int32_t vocab,
+                                      const int32_t *targets_dev, int32_t top_k, float *logprobs_dev, float *entropy_dev,
+                                      int32_t *top_ids_dev, float *top_logprobs_dev) {
+    if (int32_t rc = tlc_enter(ctx)) return rc;
+    tlc_perf_scope perf(ctx, "token_logprobs(rows=%d, vocab=%d, top=%d)", rows, vocab, top_k);
+    TLC_REQUIRE(logits_dev && (!logprobs_dev || targets_dev) && (top_k <= 0 || (top_ids_dev && top_logprobs_dev)),
+                TLC_ERR_INVALID_OPERATION, "token_logprobs: null pointer");
+    TLC_REQUIRE(rows >= 0 && rows <= INT_MAX / kMaxCluster && vocab > 0 && vocab <= INT_MAX - 8, TLC_ERR_INVALID_DIMENSION,
+                "token_logprobs: bad shape [%d, %d]", rows, vocab);
+    TLC_REQUIRE(top_k >= 0 && top_k <= kMaxTop, TLC_ERR_INVALID_OPERATION, "token_logprobs: top_k %d outside 0 .. %d", top_k, kMaxTop);
+    TLC_REQUIRE(((uintptr_t)logits_dev & 1) == 0, TLC_ERR_INVALID_OPERATION, "token_logprobs: logits must be 2-byte aligned");
+    if (rows == 0) return TLC_OK;
+    LogprobParams p{};
+    p.logits = static_cast<const __half *>(logits_dev);
+    p.targets = targets_dev;
+    p.logprobs = logprobs_dev;
+    p.entropy = entropy_dev;
+    p.top_ids = top_ids_dev;
+    p.top_logprobs = top_logprobs_dev;
+    p.rows = rows;
+    p.vocab = vocab;
+    p.top = top_k;
+    p.status = ctx->dev_status;
+    // CTAs a row: so many that each holds its slice at once, and more of them while SMs are idle and slices are long.
+    int c = 1;
+    while (c < kMaxCluster && ((long long)c * kSlice < vocab || ((long long)rows * c * 2 <= ctx->sm_count && vocab / c >= 8192))) c *= 2;
+    p.cluster = c;
+    const size_t smem = top_k > 0 ? kList * sizeof(unsigned long long) : 0;
+    static bool configured[64] = {};
+    if (!configured[ctx->device & 63]) {
+        TLC_CUDA(cudaFuncSetAttribute(logprob_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kList * sizeof(unsigned long long))));
+        configured[ctx->device & 63] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * c));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (c > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = (unsigned)c;
+        attr[na].val.clusterDim.y = 1;
+        attr[na++].val.clusterDim.z = 1;
+    }
+    if (ctx->use_pdl && ctx->pdl_small) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    const cudaError_t le = top_k > 0 ? cudaLaunchKernelEx(&cfg, logprob_kernel<true>, p) : cudaLaunchKernelEx(&cfg, logprob_kernel<false>, p);
+    if (le != cudaSuccess) {
+        cudaGetLastError();
+        return tlc_fail(TLC_ERR_CUDA, "token_logprobs launch failed: %s", cudaGetErrorString(le));
+    }
+    TLC_CHECK_LAUNCH(ctx);
+    return TLC_OK;
+}

@@ -1,0 +1,87 @@
+"""What the 8-bit KV cache and the token log probabilities refuse before anything reaches a GPU."""
+import types
+
+import numpy as np
+import pytest
+
+from tensorlogic_b200 import _lib
+from tensorlogic_b200.api import KVCache8, Tensor, token_logprobs
+
+
+class _Lib:
+    """Every call succeeds and is written down."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+@pytest.fixture
+def fake():
+    return types.SimpleNamespace(lib=_Lib(), handle=1, _slot=(1, 4096), _slot_at=0, synchronize=lambda: None)
+
+
+def _tensor(dev, shape):
+    t = Tensor.__new__(Tensor)
+    t.dev, t.shape, t.size, t.ptr, t._buf = dev, tuple(shape), int(np.prod(shape)), 4096, None
+    return t
+
+
+def test_null_context_is_refused(lib):
+    for name in ("tlc_kvcache8_create", "tlc_kvcache8_append", "tlc_kvcache8_rows", "tlc_attention8", "tlc_token_logprobs"):
+        args = [t() if t in (_lib.i32, _lib.f32) else None for t in _lib.PROTOTYPES[name][1]]
+        assert getattr(lib, name)(*args) == _lib.ERR_INVALID_OPERATION and b"null context" in lib.tlc_last_error(), name
+    assert lib.tlc_kvcache8_destroy(None) == 0
+
+
+def test_cache_refusals(fake):
+    cache = KVCache8(fake, 2, 2, 64, max_seq=100, max_batch=3)
+    one = lambda n: _tensor(fake, (n, 2, 64))  # noqa: E731
+    cache.append(0, one(40), one(40), sequence=1)
+    assert list(cache.lengths[0]) == [0, 40, 0] and not cache.lengths[1].any()
+    made = len(fake.lib.calls)
+
+    def refused(code, f, *a, **k):
+        with pytest.raises(_lib.TensorError) as e:
+            f(*a, **k)
+        assert e.value.code == code
+
+    shape, index = _lib.ERR_SHAPE_MISMATCH, _lib.ERR_INDEX
+    refused(shape, cache.append, 0, _tensor(fake, (100,)), _tensor(fake, (100,)))
+    refused(shape, cache.append, 0, one(1), one(2))
+    refused(index, cache.append, 2, one(1), one(1))
+    refused(index, cache.append, -1, one(1), one(1))
+    refused(shape, cache.append, 0, one(1), one(1), sequence=3)
+    refused(shape, cache.append, 0, one(3), one(3), sequence=1, positions=[0, 0, 0])
+    refused(index, cache.append, 0, one(1), one(1), position=1)                # a gap
+    refused(index, cache.append, 0, one(1), one(1), position=-1)
+    refused(shape, cache.append, 0, one(3), one(3), positions=[0, 40])
+    refused(index, cache.append, 0, one(3), one(3), positions=[0, 41, -1])     # a gap in one of them
+    refused(shape, cache.attention, 0, one(1), 3)
+    refused(shape, cache.attention, 0, one(1), 2, batch=0)
+    refused(shape, cache.attention, 0, one(3), 2, batch=3, sequence=1)
+    refused(index, cache.attention, 0, one(1), 2)                              # nothing there
+    refused(index, cache.attention, 0, one(2), 2, q_pos0=39, sequence=1)
+    refused(index, cache.attention, 0, one(3), 2, batch=3, positions=[-1, 40, -1])
+    refused(shape, cache.attention, 0, one(3), 2, batch=3, positions=[-1, 39])
+    refused(index, cache.layer_arrays, 5)
+    refused(shape, cache.layer_arrays, 0, 3)
+    assert len(fake.lib.calls) == made  # nothing was called
+    assert list(cache.lengths[0]) == [0, 40, 0]
+    cache.append(0, one(3), one(3), positions=[0, 20, -1])
+    assert list(cache.lengths[0]) == [1, 21, 0]
+    cache.append(0, one(5), one(5), sequence=1, position=7)
+    assert list(cache.lengths[0]) == [1, 12, 0]
+
+
+def test_logprob_refusals(fake):
+    x = _tensor(fake, (2, 10))
+    for tokens, top in (([0], 0), ([0, 10], 0), ([-2, 0], 0), ([0, 1], 33), ([0, 1], -1)):
+        with pytest.raises(_lib.TensorError):
+            token_logprobs(x, tokens, top)
+    assert not any(name == "tlc_token_logprobs" for name, _ in fake.lib.calls)
