@@ -21,6 +21,7 @@
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kTcRows = 1024;  // (query, head) rows of a KV head from which a prompt runs on tcgen05
 constexpr float kShift = 12.f;        // P is held times 2^12
 constexpr float kUp = 16777216.f;     // the codes' 2^24
 constexpr float kLog2e = 1.4426950408889634f;
@@ -431,6 +432,16 @@ extern "C" int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
     const int G = n_heads / Hkv;
     TLC_REQUIRE(batch <= 65535 && (long long)n_queries * G <= INT_MAX / 64, TLC_ERR_INVALID_DIMENSION,
                 "attention8: %d sequences of %d queries", batch, n_queries);
+    // Long prompts: on tcgen05, a sequence at a time.
+    if (!positions_dev && (long long)n_queries * G >= kTcRows && G <= 128) {
+        for (int b = 0; b < batch; b++) {
+            const size_t at = (size_t)b * n_queries * n_heads * D;
+            if (int32_t rc = kv8_attention_tc(ctx, cache, layer, sequence + b, static_cast<const __half *>(q_dev) + at,
+                                              static_cast<__half *>(out_dev) + at, n_queries, n_heads, q_pos0, scale))
+                return rc;
+        }
+        return TLC_OK;
+    }
     Params p{};
     p.q = static_cast<const __half *>(q_dev);
     p.out = static_cast<__half *>(out_dev);

@@ -35,7 +35,10 @@ struct tlc_kvcache8 {
     int *lengths;     // [layer][sequence][kv head][K, V]: rows held (a copy for each CTA that appends)
     float *partial;   // shared keys: [CTA][row][D + 2]
     int *tickets;     // zero between launches
-    __half *wide;     // codes of one layer and sequence as f16 for long prompts, made on first use
+    // Made on first use by a long prompt: the blocks of one layer and sequence as f16 rows [K, V][kv head][position][D],
+    // and per block what they count (kv8_widen).
+    __half *wide;
+    float4 *factors;
     size_t heads() const { return (size_t)max_batch * n_kv_heads; }  // of a layer
 };
 
@@ -54,6 +57,12 @@ inline Kv8View kv8_view(const tlc_kvcache8 *c, int layer, int first) {
 }
 // Argument checks that every call over the cache makes: whose it is, the layer, the sequences.
 int32_t kv8_check(tlc_ctx *ctx, const tlc_kvcache8 *cache, const char *what, int layer, int first, int sequences);
+
+// Fills wide and factors with the first `blocks` blocks of a sequence.
+int32_t kv8_widen(tlc_ctx *ctx, tlc_kvcache8 *cache, int layer, int sequence, int blocks);
+// Attention of a prompt over that image on the 5th-generation tensor cores (tlc_attention8_tc.cu).
+int32_t kv8_attention_tc(tlc_ctx *ctx, tlc_kvcache8 *cache, int layer, int sequence, const __half *q, __half *out, int I, int H,
+                         int pos0, float scale);
 
 #ifdef __CUDACC__
 // Key (0..15) that row r of a 16-key group holds, and the row that holds key j.
