@@ -1,27 +1,28 @@
 // Log probabilities of given tokens, entropy and the likeliest alternatives of logit rows, in one pass.
 //
-//   S = sum exp(x - m),  log p(t) = x_t - m - ln S,  H = ln S - sum exp(x - m) (x - m) / S,  m = max x (finite x only)
+//   log p(t) = x_t - ln sum e^x,   H = ln sum e^x - sum p x,   over the finite x of a row
 //
-// A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary that its 512 threads hold in registers
-// (64 values a thread): read once, then the maximum, then the exponentials.  x log2(e) + c with c = -m log2(e) is one
-// fused multiply-add; c is off by some delta, which multiplies all exponentials alike and is divided out at the end,
-// so that large logits lose nothing.
+// A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary.  A thread streams 16-byte pieces and
+// keeps a running s = sum 2^y, t = sum 2^y y with y = x log2(e) + c, one fused multiply-add, and c = -m log2(e) in f32
+// for the largest x so far: whatever c is rounded to, log2 p(x) = y - log2 s, so that large logits lose nothing.
 //
-// Alternatives: (value, lowest id first) is one 48-bit key per logit, so no two are equal.  The k-th largest of the best
-// keys of 128 groups of four threads is a bound that at least k logits reach, and none but those of at most k groups
-// can: these few are collected and ranked by counting.
+// Alternatives (logprob_top_kernel): the slice is held in registers, 8 to 64 values a thread, and taken once more for
+// them.  (value, lowest id first) is one 48-bit key per logit, so no two are equal.  The k-th largest of the best keys
+// of 128 groups of four threads is a bound that at least k logits reach, and none but those of at most k groups can:
+// these few are collected and ranked by counting.
 #include <cuda_fp16.h>
 
 #include "tlc_internal.h"
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kPieces = 8;  // 16-byte pieces a thread
-constexpr int kSlice = kThreads * kPieces * 8;                      // values a CTA holds at a time
-constexpr int kMaxTop = 32, kGroups = kThreads / 4;
-constexpr int kList = kMaxTop * kPieces * 8 * 4 + kMaxTop;  // what k groups hold, and the best of earlier slices
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kUnroll = 4;  // 16-byte pieces of a thread in flight, twice
+constexpr int kTopThreads = 512, kTopWarps = kTopThreads / 32, kGroups = kTopThreads / 4;
+constexpr int kMaxTop = 32, kMaxCluster = 8;
+// what k groups of threads with so many 16-byte pieces each hold, and the best of earlier passes
+template <int PIECES> constexpr int list_size() { return kMaxTop * PIECES * 8 * 4 + kMaxTop; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ float exp2_of(float x) {
     float y;
@@ -38,15 +39,203 @@ struct LogprobParams {
     tlc_dev_status *status;
 };
 struct Sums {
-    float m, s, t;  // maximum, sum of e^(x - m), sum of e^(x - m) (x - m) log2(e)
+    float c, s, t;  // c = +inf: no logits
 };
-// Those of two disjoint sets.
-__device__ __forceinline__ Sums joined(const Sums &a, const Sums &b) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return a;
-    const float da = fmaxf((a.m - m) * kLog2e, -1e30f), db = fmaxf((b.m - m) * kLog2e, -1e30f);  // (an empty set's is -inf)
-    const float wa = exp2_of(da), wb = exp2_of(db);
-    return {m, wa * a.s + wb * b.s, wa * (a.t + da * a.s) + wb * (b.t + db * b.s)};
+// s and t as they are for another c (smaller or the same).
+__device__ __forceinline__ void moved_to(Sums &a, float c) {
+    if (a.c == c) return;
+    const float d = fmaxf(c - a.c, -1e30f), w = exp2_of(d);
+    a.t = w * (a.t + d * a.s);
+    a.s *= w;
+    a.c = c;
+}
+
+// Log probability of a logit, and what a row without alternatives returns.
+__device__ __forceinline__ float logprob_of(float x, const Sums &run, float log2_s) { return (fmaf(x, kLog2e, run.c) - log2_s) * kLn2; }
+__device__ __forceinline__ void store_row(const LogprobParams &p, int row, const Sums &run) {
+    const bool any = run.c < INFINITY;
+    const float log2_s = any ? log2f(run.s) : 0.f;
+    if (p.logprobs) {
+        const int target = p.targets[row];
+        float lp = 0.f;
+        if (target >= 0 && target < p.vocab) {
+            const float x = __half2float(p.logits[(size_t)row * p.vocab + target]);
+            lp = isfinite(x) ? logprob_of(x, run, log2_s) : -INFINITY;
+        } else if (target != -1) {
+            lp = __int_as_float(0x7FC00000);
+            if (atomicCAS(&p.status->code, 0, TLC_DEV_INDEX) == 0) p.status->where = TLC_WHERE_TOKEN;
+        }
+        p.logprobs[row] = lp;
+    }
+    if (p.entropy) p.entropy[row] = any ? fmaxf((log2_s - run.t / run.s) * kLn2, 0.f) : 0.f;
+}
+// The sums of a warp's lanes, those of a CTA's warps.
+__device__ __forceinline__ void warp_sums(Sums &run) {
+    float c = run.c;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) c = fminf(c, __shfl_xor_sync(0xffffffffu, c, o));
+    moved_to(run, c);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        run.s += __shfl_xor_sync(0xffffffffu, run.s, o);
+        run.t += __shfl_xor_sync(0xffffffffu, run.t, o);
+    }
+}
+__device__ __forceinline__ void joined(Sums &run, Sums a) {
+    const float c = fminf(run.c, a.c);
+    moved_to(run, c);
+    moved_to(a, c);
+    run.s += a.s;
+    run.t += a.t;
+}
+
+// A row in the 16-byte pieces of memory it lies in: the first and the last may reach into other rows and past the array.
+struct Row {
+    const __half *base, *lo, *hi;
+    int ahead, vocab;  // values of the first piece in front of the row
+    long long pieces;
+    // Its values of a piece; -inf for what is not finite or not the row's.
+    __device__ __forceinline__ uint4 load(long long at, long long end) const {
+        uint4 w = make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
+        if (at >= end) return w;
+        const __half *src = base + at * 8;
+        if (src >= lo && src + 8 <= hi) {
+            w = *reinterpret_cast<const uint4 *>(src);
+        } else {
+            __half h[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) h[e] = src + e >= lo && src + e < hi ? src[e] : __ushort_as_half((unsigned short)0xFC00);
+#pragma unroll
+            for (int e = 0; e < 4; e++) reinterpret_cast<__half2 *>(&w)[e] = __halves2half2(h[2 * e], h[2 * e + 1]);
+        }
+        return w;
+    }
+    __device__ __forceinline__ void clean(uint4 w, long long at, __half2 (&v)[4]) const {
+        const __half2 neg_inf = __float2half2_rn(-INFINITY), neg_zero = __floats2half2_rn(-0.f, -0.f);
+        unsigned m[4] = {w.x, w.y, w.z, w.w};
+        if (at == 0 || at + 1 == pieces) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const long long i = at * 8 + 2 * e - ahead;
+                if (i < 0 || i >= vocab) m[e] = (m[e] & 0xFFFF0000u) | 0xFC00u;
+                if (i + 1 < 0 || i + 1 >= vocab) m[e] = (m[e] & 0xFFFFu) | 0xFC000000u;
+            }
+        }
+        // x * -0 + x is NaN for what is not finite, x for the rest (+0 for -0); the maximum passes over NaN
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const __half2 h = *reinterpret_cast<const __half2 *>(&m[e]);
+            v[e] = __hmax2(__hfma2(h, neg_zero, h), neg_inf);
+        }
+    }
+};
+
+// Without alternatives.
+__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParams p) {
+    __shared__ Sums sums[kMaxCluster];
+    __shared__ float warp_c[kWarps], warp_s[kWarps], warp_t[kWarps];
+    if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    tlc_pdl_after_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blockIdx.x % p.cluster, row = blockIdx.x / p.cluster;
+    const __half *x0 = p.logits + (size_t)row * p.vocab;
+    Row r;
+    r.ahead = (int)(((uintptr_t)x0 & 15) >> 1);
+    r.vocab = p.vocab;
+    r.base = x0 - r.ahead;
+    r.lo = p.logits;
+    r.hi = p.logits + (size_t)p.rows * p.vocab;
+    r.pieces = ((long long)r.ahead + p.vocab + 7) / 8;
+    const long long share = (r.pieces + p.cluster - 1) / p.cluster, first = rank * share,
+                    end = first + share < r.pieces ? first + share : r.pieces;
+
+    // ---- one pass: the thread's largest value and its sums ----
+    Sums run = {INFINITY, 0.f, 0.f};
+    float most = -INFINITY;
+    {
+        uint4 w[kUnroll];
+#pragma unroll
+        for (int i = 0; i < kUnroll; i++) w[i] = r.load(first + tid + i * kThreads, end);
+        for (long long at = first + tid; at < end; at += kUnroll * kThreads) {
+            __half2 v[kUnroll * 4];
+#pragma unroll
+            for (int i = 0; i < kUnroll; i++) {
+                __half2 u[4];
+                r.clean(w[i], at + i * kThreads, u);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[4 * i + e] = u[e];
+                w[i] = r.load(at + (kUnroll + i) * kThreads, end);
+            }
+            __half2 mx[2] = {v[0], v[1]};
+#pragma unroll
+            for (int e = 2; e < kUnroll * 4; e++) mx[e & 1] = __hmax2(mx[e & 1], v[e]);
+            mx[0] = __hmax2(mx[0], mx[1]);
+            const float m = fmaxf(__low2float(mx[0]), __high2float(mx[0]));
+            if (m > most) {
+                most = m;
+                moved_to(run, -(m * kLog2e));
+            }
+            if (most == -INFINITY) continue;
+            float s4[4] = {run.s, 0.f, 0.f, 0.f}, t4[4] = {run.t, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < kUnroll * 4; e++) {
+                const float2 f = __half22float2(v[e]);
+                // (2^-200 is zero; 2^y y of a logit of -inf would be NaN)
+                const float a = fmaxf(fmaf(f.x, kLog2e, run.c), -200.f), b = fmaxf(fmaf(f.y, kLog2e, run.c), -200.f);
+                const float ea = exp2_of(a), eb = exp2_of(b);
+                s4[2 * (e & 1)] += ea;
+                s4[2 * (e & 1) + 1] += eb;
+                t4[2 * (e & 1)] = fmaf(ea, a, t4[2 * (e & 1)]);
+                t4[2 * (e & 1) + 1] = fmaf(eb, b, t4[2 * (e & 1) + 1]);
+            }
+            run.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            run.t = (t4[0] + t4[1]) + (t4[2] + t4[3]);
+        }
+    }
+    // ---- the CTA's sums ----
+    {
+        warp_sums(run);
+        if (lane == 0) {
+            warp_c[warp] = run.c;
+            warp_s[warp] = run.s;
+            warp_t[warp] = run.t;
+        }
+    }
+    __syncthreads();
+    {
+        float c = warp_c[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; w++) c = fminf(c, warp_c[w]);
+        run = {c, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            Sums a = {warp_c[w], warp_s[w], warp_t[w]};
+            moved_to(a, c);
+            run.s += a.s;
+            run.t += a.t;
+        }
+    }
+    // ---- the first CTA of the row joins what the others found ----
+    if (p.cluster > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the row runs
+        __syncthreads();
+        auto remote = [&](const void *at) {
+            uint32_t a;
+            asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)));
+            return a;
+        };
+        if (rank > 0) {
+            if (tid < 3)
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(&sums[rank].c) + 4 * tid), "f"(tid == 0 ? run.c : tid == 1 ? run.s : run.t)
+                             : "memory");
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank > 0) return;
+        for (int i = 1; i < p.cluster; i++) joined(run, sums[i]);
+    }
+    if (tid == 0) store_row(p, row, run);
 }
 
 // Larger for a larger value, then for a smaller id; 0: no logit.
@@ -60,13 +249,14 @@ __device__ __forceinline__ __half value_of(unsigned long long key) {
     return __ushort_as_half((v & 0x8000) ? (unsigned short)(v & 0x7FFF) : (unsigned short)~v);
 }
 
-template <bool TOP>
-__global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParams p) {
-    extern __shared__ __align__(16) unsigned long long list[];  // [kList] (TOP)
+// With alternatives.
+template <int PIECES>
+__global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const LogprobParams p) {
+    extern __shared__ __align__(16) unsigned long long list[];  // [list_size<PIECES>()]
     __shared__ __align__(16) unsigned long long group_best[kGroups];
     __shared__ unsigned long long best[kMaxCluster][kMaxTop];  // of this CTA's slices; in the first CTA, of all
     __shared__ Sums sums[kMaxCluster];
-    __shared__ float warp_max[kWarps], warp_s[kWarps], warp_t[kWarps];
+    __shared__ float warp_max[kTopWarps], warp_s[kTopWarps], warp_t[kTopWarps];
     __shared__ unsigned long long bound;
     __shared__ int n_list;
     if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -80,14 +270,14 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
     const long long pieces = ((long long)ahead + p.vocab + 7) / 8, share = (pieces + p.cluster - 1) / p.cluster;
     const long long first = rank * share, end = first + share < pieces ? first + share : pieces;
 
-    if (TOP && tid < p.top) best[0][tid] = 0;
-    Sums run = {-INFINITY, 0.f, 0.f};
+    if (tid < p.top) best[0][tid] = 0;
+    Sums run = {INFINITY, 0.f, 0.f};
     const __half2 neg_inf = __float2half2_rn(-INFINITY), neg_zero = __floats2half2_rn(-0.f, -0.f);
-    for (long long p0 = first; p0 < end; p0 += kThreads * kPieces) {
-        __half2 v[kPieces * 4];
+    for (long long p0 = first; p0 < end; p0 += kTopThreads * PIECES) {
+        __half2 v[PIECES * 4];
 #pragma unroll
-        for (int i = 0; i < kPieces; i++) {
-            const long long at = p0 + tid + i * kThreads;
+        for (int i = 0; i < PIECES; i++) {
+            const long long at = p0 + tid + i * kTopThreads;
             const __half *src = base + at * 8;
             uint4 w = make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);  // -inf
             if (at < end) {
@@ -113,22 +303,22 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
         }
         __half2 mx = v[0];
 #pragma unroll
-        for (int e = 1; e < kPieces * 4; e++) mx = __hmax2(mx, v[e]);
+        for (int e = 1; e < PIECES * 4; e++) mx = __hmax2(mx, v[e]);
         const float mine = fmaxf(__low2float(mx), __high2float(mx));
         float m = mine;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         __syncthreads();  // (what the slice before left here has been read)
         if (lane == 0) warp_max[warp] = m;
-        if (TOP) {
+        {
             // this group's best key: of the values equal to a thread's maximum, the first
             unsigned long long k = 0;
             if (mine > -INFINITY) {
                 const __half want = __float2half_rn(mine);
                 unsigned id = 0;
 #pragma unroll
-                for (int e = kPieces * 4 - 1; e >= 0; e--) {
-                    const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kThreads) * 8 + 2 * (e & 3) - ahead);
+                for (int e = PIECES * 4 - 1; e >= 0; e--) {
+                    const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kTopThreads) * 8 + 2 * (e & 3) - ahead);
                     if (__heq(__high2half(v[e]), want)) id = at + 1;
                     if (__heq(__low2half(v[e]), want)) id = at;
                 }
@@ -148,8 +338,8 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
         __syncthreads();
         m = warp_max[0];
 #pragma unroll
-        for (int w = 1; w < kWarps; w++) m = fmaxf(m, warp_max[w]);
-        if (TOP) {
+        for (int w = 1; w < kTopWarps; w++) m = fmaxf(m, warp_max[w]);
+        {
             // group tid / 4, against a quarter of the others: the one with k - 1 better ones is the bound
             const unsigned long long own = group_best[tid >> 2];
             int better = 0;
@@ -160,13 +350,12 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
             if ((tid & 3) == 0 && better == p.top - 1 && own > 0) bound = own;
             if (tid < p.top) list[tid] = best[0][tid];
         }
-        float s = 0.f, t = 0.f, delta = 0.f;
+        float s = 0.f, t = 0.f;
+        const float c = -(m * kLog2e);
         if (m > -INFINITY) {
-            const float c = -(m * kLog2e);
-            delta = fmaf(m, kLog2e, c);
             float s4[4] = {0.f, 0.f, 0.f, 0.f}, t4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < kPieces * 4; e++) {
+            for (int e = 0; e < PIECES * 4; e++) {
                 const float2 f = __half22float2(v[e]);
                 // (2^-200 is zero; e t of a logit of -inf would be NaN)
                 const float a = fmaxf(fmaf(f.x, kLog2e, c), -200.f), b = fmaxf(fmaf(f.y, kLog2e, c), -200.f);
@@ -189,13 +378,13 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
             warp_t[warp] = t;
         }
         __syncthreads();
-        if (TOP) {
+        {
             const unsigned long long least = bound;  // 0: fewer than k groups have anything
             // (a thread whose maximum is below the bound's value has nothing to add)
             if (mine > -INFINITY && (least == 0 || mine >= __half2float(value_of(least)))) {
 #pragma unroll
-                for (int e = 0; e < kPieces * 4; e++) {
-                    const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kThreads) * 8 + 2 * (e & 3) - ahead);
+                for (int e = 0; e < PIECES * 4; e++) {
+                    const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kTopThreads) * 8 + 2 * (e & 3) - ahead);
                     const __half a = __low2half(v[e]), b = __high2half(v[e]);
                     if (__hgt(a, __low2half(neg_inf)) && key_of(a, at) >= least) list[atomicAdd(&n_list, 1)] = key_of(a, at);
                     if (__hgt(b, __low2half(neg_inf)) && key_of(b, at + 1) >= least) list[atomicAdd(&n_list, 1)] = key_of(b, at + 1);
@@ -204,18 +393,17 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
         }
         s = t = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) {
+        for (int w = 0; w < kTopWarps; w++) {
             s += warp_s[w];
             t += warp_t[w];
         }
-        const float back = exp2_of(-delta);
-        run = joined(run, {m, s * back, (t - delta * s) * back});
-        if (TOP) {
+        joined(run, {c, s, t});
+        {
             __syncthreads();
             const int n = n_list;
             if (tid < p.top) best[0][tid] = 0;
             __syncthreads();
-            for (int i = tid; i < n; i += kThreads) {
+            for (int i = tid; i < n; i += kTopThreads) {
                 const unsigned long long own = list[i];
                 int rank_of = 0;
                 for (int j = 0; j < n; j++) rank_of += list[j] > own;
@@ -233,38 +421,22 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
             return a;
         };
         if (rank > 0) {
-            if (TOP && tid < p.top)
+            if (tid < p.top)
                 asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&best[rank][tid])), "l"(best[0][tid]) : "memory");
             if (tid < 3)
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(&sums[rank].m) + 4 * tid), "f"(tid == 0 ? run.m : tid == 1 ? run.s : run.t)
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(&sums[rank].c) + 4 * tid), "f"(tid == 0 ? run.c : tid == 1 ? run.s : run.t)
                              : "memory");
         }
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank > 0) return;
-        for (int i = 1; i < p.cluster; i++) run = joined(run, sums[i]);
+        for (int i = 1; i < p.cluster; i++) joined(run, sums[i]);
     } else {
         __syncthreads();
     }
-    const bool any = run.m > -INFINITY;
-    const float ln_s = any ? logf(run.s) : 0.f;
-    if (tid == 0) {
-        if (p.logprobs) {
-            const int target = p.targets[row];
-            float lp = 0.f;
-            if (target >= 0 && target < p.vocab) {
-                const float x = __half2float(x0[target]);
-                lp = isfinite(x) ? (x - run.m) - ln_s : -INFINITY;
-            } else if (target != -1) {
-                lp = __int_as_float(0x7FC00000);
-                if (atomicCAS(&p.status->code, 0, TLC_DEV_INDEX) == 0) p.status->where = TLC_WHERE_TOKEN;
-            }
-            p.logprobs[row] = lp;
-        }
-        if (p.entropy) p.entropy[row] = any ? fmaxf(ln_s - kLn2 * run.t / run.s, 0.f) : 0.f;
-    }
-    if (!TOP) return;
+    if (tid == 0) store_row(p, row, run);
+    const float log2_s = run.c < INFINITY ? log2f(run.s) : 0.f;
     // Rank of each CTA's best among all of them
     const int n = p.cluster * p.top;
     if (tid < n) {
@@ -278,13 +450,27 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
         const size_t out = (size_t)row * p.top;
         if (own > 0 && rank_of < p.top) {
             p.top_ids[out + rank_of] = (int)(0xFFFFFFFFu - (unsigned)own);
-            p.top_logprobs[out + rank_of] = (__half2float(value_of(own)) - run.m) - ln_s;
+            p.top_logprobs[out + rank_of] = logprob_of(__half2float(value_of(own)), run, log2_s);
         }
         if (tid < p.top && tid >= there) {
             p.top_ids[out + tid] = -1;
             p.top_logprobs[out + tid] = -INFINITY;
         }
     }
+}
+
+template <int PIECES>
+cudaError_t launch_top(tlc_ctx *ctx, cudaLaunchConfig_t &cfg, const LogprobParams &p) {
+    constexpr size_t smem = list_size<PIECES>() * sizeof(unsigned long long);
+    static bool configured[64] = {};
+    if (!configured[ctx->device & 63]) {
+        const cudaError_t e = cudaFuncSetAttribute(logprob_top_kernel<PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        configured[ctx->device & 63] = true;
+    }
+    cfg.blockDim = dim3(kTopThreads);
+    cfg.dynamicSmemBytes = smem;
+    return cudaLaunchKernelEx(&cfg, logprob_top_kernel<PIECES>, p);
 }
 
 }  // namespace
@@ -312,20 +498,14 @@ extern "C" int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int3
     p.vocab = vocab;
     p.top = top_k;
     p.status = ctx->dev_status;
-    // CTAs a row: so many that each holds its slice at once, and more of them while SMs are idle and slices are long.
+    // CTAs a row: more of them while SMs have room and slices are long; with alternatives, where a slice of more than 32
+    // values a thread costs its CTA the second place on the SM, until slices are that short.
     int c = 1;
-    while (c < kMaxCluster && ((long long)c * kSlice < vocab || ((long long)rows * c * 2 <= ctx->sm_count && vocab / c >= 8192))) c *= 2;
+    while (c < kMaxCluster && (((long long)rows * c <= ctx->sm_count && vocab / c >= 4096) || (top_k > 0 && vocab / c > kTopThreads * 32))) c *= 2;
     p.cluster = c;
-    const size_t smem = top_k > 0 ? kList * sizeof(unsigned long long) : 0;
-    static bool configured[64] = {};
-    if (!configured[ctx->device & 63]) {
-        TLC_CUDA(cudaFuncSetAttribute(logprob_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kList * sizeof(unsigned long long))));
-        configured[ctx->device & 63] = true;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * c));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     int na = 0;
@@ -341,7 +521,11 @@ extern "C" int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int3
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    const cudaError_t le = top_k > 0 ? cudaLaunchKernelEx(&cfg, logprob_kernel<true>, p) : cudaLaunchKernelEx(&cfg, logprob_kernel<false>, p);
+    const long long values = ((long long)vocab + 14) / 8 / c + 1;  // 16-byte pieces of a slice, at most
+    const cudaError_t le = top_k == 0                  ? cudaLaunchKernelEx(&cfg, logprob_kernel, p)
+                           : values <= kTopThreads     ? launch_top<1>(ctx, cfg, p)
+                           : values <= 2 * kTopThreads ? launch_top<2>(ctx, cfg, p)
+                                                       : launch_top<4>(ctx, cfg, p);
     if (le != cudaSuccess) {
         cudaGetLastError();
         return tlc_fail(TLC_ERR_CUDA, "token_logprobs launch failed: %s", cudaGetErrorString(le));

@@ -112,7 +112,8 @@ def test_parts_on_their_own(dev):
         assert call(*a, k=top if keep[2] else 0, t=targets if keep[0] else None) == 0
         dev.synchronize()
         for o, k, w in zip(out, keep, want):
-            assert np.array_equal(o[:rows].cpu().numpy(), w) if k else (o == 7).all()
+            # (without alternatives the sums are added in another order: each is off by 2^-18 at most, see oracle())
+            assert np.allclose(o[:rows].cpu().numpy(), w, rtol=2.0 ** -16, atol=2.0 ** -17) if k else (o == 7).all()
             assert (o[rows] == 7).all()
     out = fresh()
     assert call(None, None, None, None, k=0, t=None) == 0
