@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kUnroll = 4;  // 16-byte pieces of a thread in flight, twice
+constexpr float kLow = -60000.f;  // 2^y of the lowest f16 is zero beside any value from here on
 constexpr int kTopThreads = 512, kTopWarps = kTopThreads / 32, kGroups = kTopThreads / 4;
 constexpr int kMaxTop = 32, kMaxCluster = 8;
 // what k groups of threads with so many 16-byte pieces each hold, and the best of earlier passes
@@ -52,16 +53,26 @@ __device__ __forceinline__ void moved_to(Sums &a, float c) {
 
 // Log probability of a logit, and what a row without alternatives returns.
 __device__ __forceinline__ float logprob_of(float x, const Sums &run, float log2_s) { return (fmaf(x, kLog2e, run.c) - log2_s) * kLn2; }
-__device__ __forceinline__ void store_row(const LogprobParams &p, int row, const Sums &run) {
+struct Target {  // fetched at the start: two trips to memory, one behind the other
+    int id;
+    float x;
+};
+__device__ __forceinline__ Target target_of(const LogprobParams &p, int row) {
+    Target t = {-1, 0.f};
+    if (p.logprobs) {
+        t.id = p.targets[row];
+        if (t.id >= 0 && t.id < p.vocab) t.x = __half2float(p.logits[(size_t)row * p.vocab + t.id]);
+    }
+    return t;
+}
+__device__ __forceinline__ void store_row(const LogprobParams &p, int row, const Target &t, const Sums &run) {
     const bool any = run.c < INFINITY;
     const float log2_s = any ? log2f(run.s) : 0.f;
     if (p.logprobs) {
-        const int target = p.targets[row];
         float lp = 0.f;
-        if (target >= 0 && target < p.vocab) {
-            const float x = __half2float(p.logits[(size_t)row * p.vocab + target]);
-            lp = isfinite(x) ? logprob_of(x, run, log2_s) : -INFINITY;
-        } else if (target != -1) {
+        if (t.id >= 0 && t.id < p.vocab) {
+            lp = isfinite(t.x) ? logprob_of(t.x, run, log2_s) : -INFINITY;
+        } else if (t.id != -1) {
             lp = __int_as_float(0x7FC00000);
             if (atomicCAS(&p.status->code, 0, TLC_DEV_INDEX) == 0) p.status->where = TLC_WHERE_TOKEN;
         }
@@ -110,25 +121,30 @@ struct Row {
         }
         return w;
     }
-    __device__ __forceinline__ void clean(uint4 w, long long at, __half2 (&v)[4]) const {
-        const __half2 neg_inf = __float2half2_rn(-INFINITY), neg_zero = __floats2half2_rn(-0.f, -0.f);
+    // A piece without what is not the row's: -inf in its place.
+    __device__ __forceinline__ uint4 own(uint4 w, long long at) const {
+        if (at != 0 && at + 1 != pieces) return w;
         unsigned m[4] = {w.x, w.y, w.z, w.w};
-        if (at == 0 || at + 1 == pieces) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const long long i = at * 8 + 2 * e - ahead;
-                if (i < 0 || i >= vocab) m[e] = (m[e] & 0xFFFF0000u) | 0xFC00u;
-                if (i + 1 < 0 || i + 1 >= vocab) m[e] = (m[e] & 0xFFFFu) | 0xFC000000u;
-            }
-        }
-        // x * -0 + x is NaN for what is not finite, x for the rest (+0 for -0); the maximum passes over NaN
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const __half2 h = *reinterpret_cast<const __half2 *>(&m[e]);
-            v[e] = __hmax2(__hfma2(h, neg_zero, h), neg_inf);
+            const long long i = at * 8 + 2 * e - ahead;
+            if (i < 0 || i >= vocab) m[e] = (m[e] & 0xFFFF0000u) | 0xFC00u;
+            if (i + 1 < 0 || i + 1 >= vocab) m[e] = (m[e] & 0xFFFFu) | 0xFC000000u;
         }
+        return make_uint4(m[0], m[1], m[2], m[3]);
     }
 };
+// The eight values of a piece, `none` for those that are not finite: x * -0 + x is NaN for them, x for the rest (+0 for
+// -0), and the maximum passes over NaN and -inf.
+__device__ __forceinline__ void clean(uint4 w, __half2 none, __half2 (&v)[4]) {
+    const unsigned m[4] = {w.x, w.y, w.z, w.w};
+    const __half2 neg_zero = __floats2half2_rn(-0.f, -0.f);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const __half2 h = *reinterpret_cast<const __half2 *>(&m[e]);
+        v[e] = __hmax2(__hfma2(h, neg_zero, h), none);
+    }
+}
 
 // Without alternatives.
 __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParams p) {
@@ -139,6 +155,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x % p.cluster, row = blockIdx.x / p.cluster;
     const __half *x0 = p.logits + (size_t)row * p.vocab;
+    Target target = {-1, 0.f};
+    if (tid == 0 && rank == 0) target = target_of(p, row);
     Row r;
     r.ahead = (int)(((uintptr_t)x0 & 15) >> 1);
     r.vocab = p.vocab;
@@ -153,35 +171,62 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
     Sums run = {INFINITY, 0.f, 0.f};
     float most = -INFINITY;
     {
+        // 1024 pieces a turn.  Turns within the row need no look at its ends.
+        constexpr int kTurn = kUnroll * kThreads;
         uint4 w[kUnroll];
+        auto inside = [&](long long turn) { return turn > 0 && turn + kTurn < r.pieces && turn + kTurn <= end; };
+        auto load = [&](long long turn) {
+            if (inside(turn)) {
 #pragma unroll
-        for (int i = 0; i < kUnroll; i++) w[i] = r.load(first + tid + i * kThreads, end);
-        for (long long at = first + tid; at < end; at += kUnroll * kThreads) {
+                for (int i = 0; i < kUnroll; i++) w[i] = *reinterpret_cast<const uint4 *>(r.base + (turn + tid + i * kThreads) * 8);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kUnroll; i++) w[i] = r.load(turn + tid + i * kThreads, end);
+            }
+        };
+        load(first);
+        for (long long turn = first; turn < end; turn += kTurn) {
+            if (!inside(turn)) {
+#pragma unroll
+                for (int i = 0; i < kUnroll; i++) w[i] = r.own(w[i], turn + tid + i * kThreads);
+            }
+            // What is not finite becomes the lowest f16, which counts for nothing beside a larger value; a turn that
+            // has none (below, the rare case) is looked at value by value.
             __half2 v[kUnroll * 4];
 #pragma unroll
-            for (int i = 0; i < kUnroll; i++) {
-                __half2 u[4];
-                r.clean(w[i], at + i * kThreads, u);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[4 * i + e] = u[e];
-                w[i] = r.load(at + (kUnroll + i) * kThreads, end);
-            }
+            for (int i = 0; i < kUnroll; i++) clean(w[i], __float2half2_rn(-65504.f), *reinterpret_cast<__half2(*)[4]>(&v[4 * i]));
+            if (turn + kTurn < end) load(turn + kTurn);
             __half2 mx[2] = {v[0], v[1]};
 #pragma unroll
             for (int e = 2; e < kUnroll * 4; e++) mx[e & 1] = __hmax2(mx[e & 1], v[e]);
             mx[0] = __hmax2(mx[0], mx[1]);
             const float m = fmaxf(__low2float(mx[0]), __high2float(mx[0]));
+            if (fmaxf(m, most) < kLow) {
+#pragma unroll 1
+                for (int i = 0; i < kUnroll * 8; i++) {
+                    const long long at = turn + tid + (i >> 3) * kThreads, n = at * 8 + (i & 7) - r.ahead;
+                    if (at >= end || n < 0 || n >= r.vocab) continue;
+                    const float x = __half2float(r.base[at * 8 + (i & 7)]);
+                    if (!isfinite(x)) continue;
+                    if (x > most) {
+                        most = x;
+                        moved_to(run, -(x * kLog2e));
+                    }
+                    const float y = fmaf(x, kLog2e, run.c), e = exp2_of(y);
+                    run.s += e;
+                    run.t = fmaf(e, y, run.t);
+                }
+                continue;
+            }
             if (m > most) {
                 most = m;
                 moved_to(run, -(m * kLog2e));
             }
-            if (most == -INFINITY) continue;
             float s4[4] = {run.s, 0.f, 0.f, 0.f}, t4[4] = {run.t, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < kUnroll * 4; e++) {
                 const float2 f = __half22float2(v[e]);
-                // (2^-200 is zero; 2^y y of a logit of -inf would be NaN)
-                const float a = fmaxf(fmaf(f.x, kLog2e, run.c), -200.f), b = fmaxf(fmaf(f.y, kLog2e, run.c), -200.f);
+                const float a = fmaf(f.x, kLog2e, run.c), b = fmaf(f.y, kLog2e, run.c);
                 const float ea = exp2_of(a), eb = exp2_of(b);
                 s4[2 * (e & 1)] += ea;
                 s4[2 * (e & 1) + 1] += eb;
@@ -235,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
         if (rank > 0) return;
         for (int i = 1; i < p.cluster; i++) joined(run, sums[i]);
     }
-    if (tid == 0) store_row(p, row, run);
+    if (tid == 0) store_row(p, row, target, run);
 }
 
 // Larger for a larger value, then for a smaller id; 0: no logit.
@@ -247,6 +292,23 @@ __device__ __forceinline__ unsigned long long key_of(__half x, unsigned id) {
 __device__ __forceinline__ __half value_of(unsigned long long key) {
     const unsigned short v = (unsigned short)(key >> 32);
     return __ushort_as_half((v & 0x8000) ? (unsigned short)(v & 0x7FFF) : (unsigned short)~v);
+}
+
+// take(key, its index, how many are larger) for those of n keys (not 0) that fewer than `top` are larger than: up to 32
+// threads a key.
+template <typename F>
+__device__ __forceinline__ void ranked(const unsigned long long *keys, int n, int top, F &&take) {
+    int lanes = 32;
+    while (lanes > 1 && lanes * n > kTopThreads) lanes >>= 1;
+    const int sub = threadIdx.x & (lanes - 1), step = kTopThreads / lanes;
+    for (int i0 = 0; i0 < n; i0 += step) {
+        const int i = i0 + threadIdx.x / lanes;
+        const unsigned long long key = i < n ? keys[i] : 0;
+        int above = 0;
+        for (int j = sub; j < n; j += lanes) above += keys[j] > key;
+        for (int o = 1; o < lanes; o *= 2) above += __shfl_xor_sync(0xffffffffu, above, o);
+        if (sub == 0 && key > 0 && above < top) take(key, i, above);
+    }
 }
 
 // With alternatives.
@@ -264,6 +326,8 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x % p.cluster, row = blockIdx.x / p.cluster;
     const __half *x0 = p.logits + (size_t)row * p.vocab;
+    Target target = {-1, 0.f};
+    if (tid == 0 && rank == 0) target = target_of(p, row);
     // The row in 16-byte pieces of memory: the first and the last may reach into other rows, and past the array.
     const int ahead = (int)(((uintptr_t)x0 & 15) >> 1);  // values of the first piece in front of the row
     const __half *base = x0 - ahead, *lo = p.logits, *hi = p.logits + (size_t)p.rows * p.vocab;
@@ -381,13 +445,17 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
         {
             const unsigned long long least = bound;  // 0: fewer than k groups have anything
             // (a thread whose maximum is below the bound's value has nothing to add)
-            if (mine > -INFINITY && (least == 0 || mine >= __half2float(value_of(least)))) {
+            const __half least_x = least ? value_of(least) : __ushort_as_half((unsigned short)0xFBFF);  // the lowest f16
+            if (mine >= __half2float(least_x)) {
+                const __half2 least2 = __half2half2(least_x);
 #pragma unroll
                 for (int e = 0; e < PIECES * 4; e++) {
+                    const unsigned hit = __hge2_mask(v[e], least2);
+                    if (hit == 0) continue;
                     const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kTopThreads) * 8 + 2 * (e & 3) - ahead);
-                    const __half a = __low2half(v[e]), b = __high2half(v[e]);
-                    if (__hgt(a, __low2half(neg_inf)) && key_of(a, at) >= least) list[atomicAdd(&n_list, 1)] = key_of(a, at);
-                    if (__hgt(b, __low2half(neg_inf)) && key_of(b, at + 1) >= least) list[atomicAdd(&n_list, 1)] = key_of(b, at + 1);
+                    const unsigned long long a = key_of(__low2half(v[e]), at), b = key_of(__high2half(v[e]), at + 1);
+                    if ((hit & 0xFFFFu) && a >= least) list[atomicAdd(&n_list, 1)] = a;
+                    if (hit >> 16 && b >= least) list[atomicAdd(&n_list, 1)] = b;
                 }
             }
         }
@@ -403,12 +471,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
             const int n = n_list;
             if (tid < p.top) best[0][tid] = 0;
             __syncthreads();
-            for (int i = tid; i < n; i += kTopThreads) {
-                const unsigned long long own = list[i];
-                int rank_of = 0;
-                for (int j = 0; j < n; j++) rank_of += list[j] > own;
-                if (own > 0 && rank_of < p.top) best[0][rank_of] = own;
-            }
+            ranked(list, n, p.top, [&](unsigned long long key, int i, int above) { best[0][above] = key; });
         }
     }
     // The first CTA of the row joins what the others found.
@@ -435,28 +498,22 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     } else {
         __syncthreads();
     }
-    if (tid == 0) store_row(p, row, run);
+    if (tid == 0) store_row(p, row, target, run);
     const float log2_s = run.c < INFINITY ? log2f(run.s) : 0.f;
-    // Rank of each CTA's best among all of them
+    // the best of all CTAs' best, which lie end to end
     const int n = p.cluster * p.top;
-    if (tid < n) {
-        const unsigned long long own = best[tid / p.top][tid % p.top];
-        int rank_of = 0, there = 0;
-        for (int c = 0; c < p.cluster; c++)
-            for (int j = 0; j < p.top; j++) {
-                rank_of += best[c][j] > own;
-                there += best[c][j] > 0;
-            }
-        const size_t out = (size_t)row * p.top;
-        if (own > 0 && rank_of < p.top) {
-            p.top_ids[out + rank_of] = (int)(0xFFFFFFFFu - (unsigned)own);
-            p.top_logprobs[out + rank_of] = logprob_of(__half2float(value_of(own)), run, log2_s);
-        }
-        if (tid < p.top && tid >= there) {
-            p.top_ids[out + tid] = -1;
-            p.top_logprobs[out + tid] = -INFINITY;
-        }
+    const size_t out = (size_t)row * p.top;
+    __syncthreads();
+    for (int i = tid; i < n; i += kTopThreads) list[i] = best[i / p.top][i % p.top];
+    if (tid < p.top) {
+        p.top_ids[out + tid] = -1;
+        p.top_logprobs[out + tid] = -INFINITY;
     }
+    __syncthreads();
+    ranked(list, n, p.top, [&](unsigned long long key, int i, int above) {
+        p.top_ids[out + above] = (int)(0xFFFFFFFFu - (unsigned)key);
+        p.top_logprobs[out + above] = logprob_of(__half2float(value_of(key)), run, log2_s);
+    });
 }
 
 template <int PIECES>
