@@ -5,15 +5,16 @@
 // On sealed blocks k_j = s_k c_j and v_j = s_v c_j with integer codes c and one scale per block, so the tensor cores
 // multiply the codes as they are (exact in f16) and s_k multiplies a score, s_v a block's product.
 //
-// attention8_kernel: a CTA of four warps owns 8 * NT (query, head) rows that share a KV head, queries in the order
-// (position, head of the group), and every nsplit-th quad of blocks; a warp takes one block at a time, alone:
+// attention8_kernel: an item is 8 * NT (query, head) rows that share a KV head, queries in the order (position, head of
+// the group).  One, two or four warps of a CTA, or those of several CTAs, share its blocks; a warp takes one at a time,
+// alone:
 //   S^T = K.Q^T  16 keys x 8 rows a product, codes as the 16-row operand (PRMT makes it, tlc_kv8.h)
 //   P            f32 maximum and sums over the keys of a row, P rounded to f16, times 2^12 so that small
 //                probabilities keep their bits; the sum is of the rounded values
 //   O^T += V^T.P P turned over by movmatrix, f32 accumulators of the block, scaled by s_v when they join O
 // A warp's blocks arrive by cp.async in a ring of its own; a lane copies the very bytes it will use, so a warp needs no
-// barrier and no other lane until the CTA's four results are merged in shared memory.  Where keys are shared out over
-// CTAs they leave (maximum, sum, O) in the cache's workspace and the last one (a ticket) merges.
+// barrier and no other lane until the results of an item's warps are merged in shared memory.  Where several CTAs share
+// its keys they leave (maximum, sum, O) in the cache's workspace and the last one (a ticket) merges.
 #include <cuda_fp16.h>
 
 #include "tlc_kv8.h"
@@ -36,7 +37,8 @@ struct Params {
     const int *positions;  // device int32[batch]: position of each sequence's query; negative: none
     int key_limit;         // keys the launch was sized for
     float scale;
-    int row_tiles, nsplit;
+    int items, row_tiles;
+    int warps, nsplit;  // warps of a CTA per item (1, 2, 4), CTAs per item (more than one: of four warps)
     float *partial;  // [CTA][row][2], then [CTA][row][D]
     int *tickets;
     tlc_dev_status *status;
@@ -77,36 +79,44 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     __shared__ int sm_last;
     tlc_pdl_after_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % p.nsplit, rt = blockIdx.x / p.nsplit, hk = blockIdx.y, b = blockIdx.z;
+    const int warps = p.warps, sub = warp % warps, gtid = sub * 32 + lane, threads = 32 * warps;
+    const int item = p.nsplit > 1 ? blockIdx.x / p.nsplit : blockIdx.x * (kWarps / warps) + warp / warps;
+    if (item >= p.items) return;
+    const int split = p.nsplit > 1 ? blockIdx.x % p.nsplit : 0;
+    const int rt = item % p.row_tiles, hk = item / p.row_tiles % p.c.n_kv_heads, b = item / p.row_tiles / p.c.n_kv_heads;
+    auto barrier = [&]() {  // of the item's warps of this CTA
+        if (warps == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / warps), "r"(threads) : "memory");
+    };
     const int rows = p.I * p.G, r0 = rt * ROWS;
     const size_t head = (size_t)b * p.c.n_kv_heads + hk;
     auto row_of = [&](int r) { return ((size_t)b * p.I + r / p.G) * p.H + hk * p.G + r % p.G; };
 
     const int at0 = p.positions ? p.positions[b] : p.pos0, held = p.c.lengths[head * 2];
     const int keys = min(held, p.key_limit);  // what a row may see at most
-    if (at0 >= 0 && at0 > keys - p.I && tid == 0 && split == 0 && atomicCAS(&p.status->code, 0, TLC_DEV_INDEX) == 0)
+    if (at0 >= 0 && at0 > keys - p.I && gtid == 0 && split == 0 && atomicCAS(&p.status->code, 0, TLC_DEV_INDEX) == 0)
         p.status->where = 400 + b;  // a query in front of its key: it sees what there is, and that is said
     const int pos0 = min(at0, keys);
     const int last = min(rows, r0 + ROWS) - 1;  // last row of the tile
     const int seen = pos0 < 0 ? 0 : min(keys, pos0 + last / p.G + 1);
     if (seen <= 0) {  // an idle slot, or nothing in the cache
         if (split == 0)
-            for (int i = tid; i < (last - r0 + 1) * (D / 8); i += kThreads)
+            for (int i = gtid; i < (last - r0 + 1) * (D / 8); i += threads)
                 *reinterpret_cast<uint4 *>(p.out + row_of(r0 + i / (D / 8)) * D + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
         return;
     }
     const int units = (seen + kKv8Block - 1) / kKv8Block, sealed = held / kKv8Block;
-    const int stride = p.nsplit * kWarps, u0 = split * kWarps + warp;
+    const int stride = p.nsplit * warps, u0 = split * warps + sub;
     const uint8_t *codes = p.c.codes + head * p.c.n_blocks * (2 * STAGE);
     const float *scales = p.c.scales + head * p.c.n_blocks * 2;
 
     // The ring: K and V of a block in turn.
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)(warp * ST * STAGE + lane * 16);
-    const int n_sealed = min(units, sealed), items = u0 < n_sealed ? 2 * ((n_sealed - u0 + stride - 1) / stride) : 0;
-    auto fetch = [&](int item) {
-        if (item < items) {
-            const uint8_t *src = codes + ((size_t)(u0 + (item >> 1) * stride) * 2 + (item & 1)) * STAGE + lane * 16;
-            const uint32_t dst = ring + (uint32_t)(item % ST * STAGE);
+    const int n_sealed = min(units, sealed), steps = u0 < n_sealed ? 2 * ((n_sealed - u0 + stride - 1) / stride) : 0;
+    auto fetch = [&](int n) {
+        if (n < steps) {
+            const uint8_t *src = codes + ((size_t)(u0 + (n >> 1) * stride) * 2 + (n & 1)) * STAGE + lane * 16;
+            const uint32_t dst = ring + (uint32_t)(n % ST * STAGE);
 #pragma unroll
             for (int i = 0; i < LOADS; i++) copy16(dst + i * 512, src + i * 512);
         }
@@ -204,14 +214,14 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
         for (int e = 0; e < 4; e++) o[nt][dt][e] = o[nt][dt][e] * corr[nt][e & 1] + acc[e] * factor;
     };
 
-    int item = 0;
+    int step = 0;
     for (int u = u0; u < n_sealed; u += stride) {
         const float sk = scales[2 * u], sv = scales[2 * u + 1];
         float s[4][NT][4], psum[NT][2], corr[NT][2];
         uint32_t pf[4][NT][2];
-        fetch(item + ST - 1);
+        fetch(step + ST - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-        uint32_t at = ring + (uint32_t)(item % ST * STAGE);
+        uint32_t at = ring + (uint32_t)(step % ST * STAGE);
 #pragma unroll
         for (int kg = 0; kg < 4; kg++) {
 #pragma unroll
@@ -229,11 +239,11 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
                 }
             }
         }
-        item++;
+        step++;
         softmax(u, s, kUp * sk * p.scale * kLog2e, pf, psum, corr);
-        fetch(item + ST - 1);
+        fetch(step + ST - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-        at = ring + (uint32_t)(item % ST * STAGE);
+        at = ring + (uint32_t)(step % ST * STAGE);
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
             float acc[2][NT][4];
@@ -256,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
                 join(2 * c + 1, nt, acc[1][nt], kUp * sv, corr);
             }
         }
-        item++;
+        step++;
     }
     // The open block, where this warp's turn has come to it: f16 rows straight from memory.
     if (units > sealed && sealed % stride == u0) {
@@ -291,9 +301,29 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();  // the ring's place takes the four warps' O: [warp][row][D], rows PITCH apart
-
-    float *so = reinterpret_cast<float *>(smem);
+    if (warps == 1 && p.nsplit == 1) {
+        // Nobody to merge with: O of rows 2t, 2t + 1 by their sums, turned over, two values of d a lane of row g.
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const float inv[2] = {1.0f / l_run[nt][0], 1.0f / l_run[nt][1]};
+            const int r = r0 + 8 * nt + g;
+            __half *to = p.out + row_of(min(r, rows - 1)) * D + 2 * t;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const __half2 v = __floats2half2_rn(o[nt][i][2 * h] * inv[0], o[nt][i][2 * h + 1] * inv[1]);
+                    const uint32_t w = turned(*reinterpret_cast<const uint32_t *>(&v));
+                    if (r < rows) *reinterpret_cast<uint32_t *>(to + 16 * i + 8 * h) = w;
+                }
+        }
+        return;
+    }
+    // A warp's O takes its ring's place: [row][D], rows PITCH apart.
+    static_assert(ROWS * PITCH * 4 <= ST * STAGE, "O in the place of the ring");
+    auto o_of = [&](int w) { return reinterpret_cast<float *>(smem + w * ST * STAGE); };
+    __syncwarp();
+    float *so = o_of(warp);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         if (g == 0) {
@@ -306,14 +336,15 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
 #pragma unroll
         for (int i = 0; i < D / 16; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) so[(warp * ROWS + 8 * nt + 2 * t + (e & 1)) * PITCH + 16 * i + g + 8 * (e >> 1)] = o[nt][i][e];
+            for (int e = 0; e < 4; e++) so[(8 * nt + 2 * t + (e & 1)) * PITCH + 16 * i + g + 8 * (e >> 1)] = o[nt][i][e];
     }
-    __syncthreads();
+    barrier();
 
     // 16 threads a row, PER values each
     constexpr int PER = D / 16;
-    const size_t slot = (((size_t)b * p.c.n_kv_heads + hk) * p.row_tiles + rt) * p.nsplit;
+    const size_t slot = (size_t)item * p.nsplit;
     float *part_ml = p.partial, *part_o = p.partial + (size_t)kKv8MaxCtas * kKv8MaxRows * 2;
+    auto weight = [](float m, float l, float M) { return m == -INFINITY && l == 0.f ? 0.f : exp2_of(m - (M == -INFINITY ? 0.f : M)); };
     auto store = [&](int r, int d0, const float (&acc)[PER], float l) {
         if (r0 + r >= rows) return;
         const float inv = 1.0f / l;  // (the largest p is 2^12; a row whose scores are NaN stays NaN)
@@ -324,60 +355,79 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
         if constexpr (PER == 8) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(h);
         else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(h);
     };
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int r = 8 * nt + (tid >> 4), d0 = (tid & 15) * PER;
+    const int w0 = warp - sub;
+    for (int r = gtid >> 4; r < ROWS; r += threads >> 4) {
+        const int d0 = (gtid & 15) * PER;
         float M = -INFINITY, L = 0.f, acc[PER];
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) M = fmaxf(M, sm_m[w][r]);
+        for (int w = 0; w < warps; w++) M = fmaxf(M, sm_m[w0 + w][r]);
 #pragma unroll
         for (int i = 0; i < PER; i++) acc[i] = 0.f;
+        for (int w = 0; w < warps; w++) {
+            const float wgt = weight(sm_m[w0 + w][r], sm_l[w0 + w][r], M);
+            L += sm_l[w0 + w][r] * wgt;
+            const float *ow = o_of(w0 + w) + r * PITCH + d0;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            const float wgt = sm_m[w][r] == -INFINITY && sm_l[w][r] == 0.f ? 0.f : exp2_of(sm_m[w][r] - (M == -INFINITY ? 0.f : M));
-            L += sm_l[w][r] * wgt;
-#pragma unroll
-            for (int i = 0; i < PER; i++) acc[i] += so[(w * ROWS + r) * PITCH + d0 + i] * wgt;
+            for (int i = 0; i < PER; i += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(ow + i);
+                acc[i] += v.x * wgt;
+                acc[i + 1] += v.y * wgt;
+                acc[i + 2] += v.z * wgt;
+                acc[i + 3] += v.w * wgt;
+            }
         }
         if (p.nsplit == 1) {
             store(r, d0, acc, L);
             continue;
         }
         const size_t at = (slot + split) * ROWS + r;
-        if ((tid & 15) == 0) *reinterpret_cast<float2 *>(part_ml + at * 2) = make_float2(M, L);
+        if ((gtid & 15) == 0) *reinterpret_cast<float2 *>(part_ml + at * 2) = make_float2(M, L);
 #pragma unroll
         for (int i = 0; i < PER; i += 4)
             *reinterpret_cast<float4 *>(part_o + at * D + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
     }
     if (p.nsplit == 1) return;
+    // (all four warps of the CTA are this item's from here on)
     __threadfence();
     __syncthreads();
     if (tid == 0) {
-        int *ticket = p.tickets + slot / p.nsplit;
+        int *ticket = p.tickets + item;
         sm_last = atomicAdd(ticket, 1) == p.nsplit - 1;
         if (sm_last) *ticket = 0;
     }
     __syncthreads();
     if (!sm_last) return;
     __threadfence();
+    // The last CTA: the splits' (maximum, sum) first, all at once, then O with several loads in flight (a chain of
+    // trips to the L2 otherwise: 74 splits took 16 us of 27).
+    float2 *ml = reinterpret_cast<float2 *>(smem);  // [split][row]
+    for (int i = tid; i < p.nsplit * ROWS; i += kThreads) ml[i] = __ldcg(reinterpret_cast<const float2 *>(part_ml + (slot * ROWS + i) * 2));
+    __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int r = 8 * nt + (tid >> 4), d0 = (tid & 15) * PER;
-        const size_t at = slot * ROWS + r;
+        const int r = 8 * nt + (tid >> 4), t16 = tid & 15, d0 = t16 * PER;
         float M = -INFINITY, L = 0.f, acc[PER];
-#pragma unroll 8
-        for (int sp = 0; sp < p.nsplit; sp++) M = fmaxf(M, __ldcg(part_ml + (at + (size_t)sp * ROWS) * 2));
+        for (int sp = t16; sp < p.nsplit; sp += 16) M = fmaxf(M, ml[sp * ROWS + r].x);
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+        for (int sp = t16; sp < p.nsplit; sp += 16) {
+            const float2 v = ml[sp * ROWS + r];
+            const float wgt = weight(v.x, v.y, M);
+            L += v.y * wgt;
+            ml[sp * ROWS + r].x = wgt;
+        }
+        // (in the order of a tree over the sixteen threads: the same for every call)
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) L += __shfl_xor_sync(0xffffffffu, L, d);
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < PER; i++) acc[i] = 0.f;
-#pragma unroll 4
+        const float *from = part_o + (slot * ROWS + r) * D + d0;
+#pragma unroll 8
         for (int sp = 0; sp < p.nsplit; sp++) {
-            const size_t a = at + (size_t)sp * ROWS;
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_ml + a * 2));
-            const float wgt = ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2_of(ml.x - (M == -INFINITY ? 0.f : M));
-            L += ml.y * wgt;
+            const float wgt = ml[sp * ROWS + r].x;
 #pragma unroll
             for (int i = 0; i < PER; i += 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_o + a * D + d0 + i));
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + (size_t)sp * (ROWS * D) + i));
                 acc[i] += v.x * wgt;
                 acc[i + 1] += v.y * wgt;
                 acc[i + 2] += v.z * wgt;
@@ -389,9 +439,10 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
 }
 
 template <int D, int NT>
-int32_t launch(tlc_ctx *ctx, const Params &p, dim3 grid) {
-    constexpr size_t ring = (size_t)kWarps * stages<D>() * kKv8Block * D, merge = (size_t)kWarps * 8 * NT * (D + 4) * sizeof(float);
-    constexpr size_t smem = ring > merge ? ring : merge;
+int32_t launch(tlc_ctx *ctx, const Params &p) {
+    constexpr size_t smem = (size_t)kWarps * stages<D>() * kKv8Block * D;
+    static_assert(smem >= (size_t)kKv8MaxCtas * 8 * NT * sizeof(float2) / 2, "the merge's maxima and sums");
+    const dim3 grid((unsigned)(p.nsplit > 1 ? p.items * p.nsplit : (p.items + kWarps / p.warps - 1) / (kWarps / p.warps)));
     static bool configured[64] = {};
     if (!configured[ctx->device & 63]) {
         TLC_CUDA(cudaFuncSetAttribute(attention8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -406,6 +457,26 @@ int32_t launch(tlc_ctx *ctx, const Params &p, dim3 grid) {
     }
     TLC_CHECK_LAUNCH(ctx);
     return TLC_OK;
+}
+
+// Warps that share an item of `units` blocks: the fewest microseconds of
+//   blocks of a warp x (the larger of a block's latency and its share of the HBM, 44 KB/us for the warps of an SM),
+// as often as the SM's eight warps have to be filled, and the merge, in shared memory or through the L2.
+void share_out(const tlc_ctx *ctx, int D, int units, Params &p) {
+    const double latency = D == 64 ? 0.45 : 0.7, share = kKv8Block * D * 2 / 44e3;
+    double best = 1e30;
+    for (int w = 1; w <= 4 * kKv8MaxCtas; w = w < 4 ? 2 * w : w + 4) {
+        const int nsplit = w <= kWarps ? 1 : w / kWarps;
+        if (w > 1 && (w > units + 3 || (nsplit > 1 && (p.items > kKv8Tickets || (long long)p.items * nsplit > kKv8MaxCtas || nsplit > kKv8MaxCtas / 2)))) break;
+        const long long per_sm = ((long long)p.items * w + ctx->sm_count - 1) / ctx->sm_count, rounds = (per_sm + 7) / 8;
+        const double at_once = (double)(per_sm < 8 ? per_sm : 8), block = latency > at_once * share ? latency : at_once * share;
+        const double t = (double)rounds * ((units + w - 1) / w) * block + (w == 1 ? 0.0 : w <= kWarps ? 0.7 : 3.0 + 0.02 * nsplit);
+        if (t < best) {
+            best = t;
+            p.warps = w < kWarps ? w : kWarps;
+            p.nsplit = nsplit;
+        }
+    }
 }
 
 }  // namespace
@@ -458,14 +529,10 @@ extern "C" int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
     p.status = ctx->dev_status;
     const int nt = n_queries * G > 8 ? 2 : 1;
     p.row_tiles = (n_queries * G + 8 * nt - 1) / (8 * nt);
-    // Keys are shared out until there are two CTAs an SM, and no further than a block a warp.
-    const long long groups = (long long)batch * Hkv * p.row_tiles, units = (T + kKv8Block - 1) / kKv8Block;
-    long long nsplit = (2 * ctx->sm_count + groups - 1) / groups;
-    if (nsplit > (units + kWarps - 1) / kWarps) nsplit = (units + kWarps - 1) / kWarps;
-    if (nsplit < 1 || groups > kKv8Tickets) nsplit = 1;
-    while (nsplit > 1 && groups * nsplit > kKv8MaxCtas) nsplit--;
-    p.nsplit = (int)nsplit;
-    const dim3 grid((unsigned)(p.row_tiles * nsplit), (unsigned)Hkv, (unsigned)batch);
-    if (D == 64) return nt == 1 ? launch<64, 1>(ctx, p, grid) : launch<64, 2>(ctx, p, grid);
-    return nt == 1 ? launch<128, 1>(ctx, p, grid) : launch<128, 2>(ctx, p, grid);
+    const long long items = (long long)batch * Hkv * p.row_tiles;
+    TLC_REQUIRE(items <= INT_MAX, TLC_ERR_INVALID_DIMENSION, "attention8: %d sequences of %d queries", batch, n_queries);
+    p.items = (int)items;
+    share_out(ctx, D, (int)((T + kKv8Block - 1) / kKv8Block), p);
+    if (D == 64) return nt == 1 ? launch<64, 1>(ctx, p) : launch<64, 2>(ctx, p);
+    return nt == 1 ? launch<128, 1>(ctx, p) : launch<128, 2>(ctx, p);
 }
