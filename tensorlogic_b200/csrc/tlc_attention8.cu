@@ -13,8 +13,10 @@
 //                probabilities keep their bits; the sum is of the rounded values
 //   O^T += V^T.P P turned over by movmatrix, f32 accumulators of the block, scaled by s_v when they join O
 // A warp's blocks arrive by cp.async in a ring of its own; a lane copies the very bytes it will use, so a warp needs no
-// barrier and no other lane until the results of an item's warps are merged in shared memory.  Where several CTAs share
-// its keys they leave (maximum, sum, O) in the cache's workspace and the last one (a ticket) merges.
+// barrier and no other lane until the results of an item's warps are merged in shared memory.  CTAs that share its keys
+// form clusters of up to eight: between two cluster barriers each takes some of the rows and pulls the others' results
+// (distributed shared memory); of several clusters the last one (a ticket for each share of the rows) joins what all have
+// left in the cache's workspace.
 #include <cuda_fp16.h>
 
 #include "tlc_kv8.h"
@@ -39,7 +41,8 @@ struct Params {
     float scale;
     int items, row_tiles;
     int warps, nsplit;  // warps of a CTA per item (1, 2, 4), CTAs per item (more than one: of four warps)
-    float *partial;  // [CTA][row][2], then [CTA][row][D]
+    int cluster;        // CTAs of a cluster: nsplit if that is 1, 2, 4 or 8, else 8
+    float *partial;  // of several clusters: [cluster][row][2], then [cluster][row][D]
     int *tickets;
     tlc_dev_status *status;
 };
@@ -75,7 +78,7 @@ template <int D, int NT>
 __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     constexpr int ROWS = 8 * NT, STAGE = kKv8Block * D, ST = stages<D>(), LOADS = STAGE / 512, PITCH = D + 4;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
+    __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];  // in a cluster: of the CTA in [0], for its peers
     __shared__ int sm_last;
     tlc_pdl_after_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     const int units = (seen + kKv8Block - 1) / kKv8Block, sealed = held / kKv8Block;
     const int stride = p.nsplit * warps, u0 = split * warps + sub;
     const uint8_t *codes = p.c.codes + head * p.c.n_blocks * (2 * STAGE);
-    const float *scales = p.c.scales + head * p.c.n_blocks * 2;
+    const float2 *scales = reinterpret_cast<const float2 *>(p.c.scales) + head * p.c.n_blocks;
 
     // The ring: K and V of a block in turn.
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)(warp * ST * STAGE + lane * 16);
@@ -122,6 +125,7 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
         }
         asm volatile("cp.async.commit_group;" ::: "memory");  // (empty ones keep the count)
     };
+    const float2 first = u0 < n_sealed ? scales[u0] : make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < ST - 1; i++) fetch(i);
 
@@ -215,8 +219,10 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     };
 
     int step = 0;
+    float2 factor = first;
     for (int u = u0; u < n_sealed; u += stride) {
-        const float sk = scales[2 * u], sv = scales[2 * u + 1];
+        const float sk = factor.x, sv = factor.y;
+        if (u + stride < n_sealed) factor = scales[u + stride];  // the next block's, a trip to memory ahead
         float s[4][NT][4], psum[NT][2], corr[NT][2];
         uint32_t pf[4][NT][2];
         fetch(step + ST - 1);
@@ -340,108 +346,149 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     }
     barrier();
 
-    // 16 threads a row, PER values each
-    constexpr int PER = D / 16;
-    const size_t slot = (size_t)item * p.nsplit;
-    float *part_ml = p.partial, *part_o = p.partial + (size_t)kKv8MaxCtas * kKv8MaxRows * 2;
     auto weight = [](float m, float l, float M) { return m == -INFINITY && l == 0.f ? 0.f : exp2_of(m - (M == -INFINITY ? 0.f : M)); };
-    auto store = [&](int r, int d0, const float (&acc)[PER], float l) {
+    auto add = [](float4 &acc, const float4 &v, float w) {
+        acc.x = fmaf(v.x, w, acc.x), acc.y = fmaf(v.y, w, acc.y), acc.z = fmaf(v.z, w, acc.z), acc.w = fmaf(v.w, w, acc.w);
+    };
+    auto store = [&](int r, int q, const float4 &acc, float l) {
         if (r0 + r >= rows) return;
         const float inv = 1.0f / l;  // (the largest p is 2^12; a row whose scores are NaN stays NaN)
-        __align__(16) __half h[PER];
-#pragma unroll
-        for (int i = 0; i < PER; i++) h[i] = __float2half_rn(acc[i] * inv);
-        __half *to = p.out + row_of(r0 + r) * D + d0;
-        if constexpr (PER == 8) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(h);
-        else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(h);
+        __align__(8) __half2 h[2] = {__floats2half2_rn(acc.x * inv, acc.y * inv), __floats2half2_rn(acc.z * inv, acc.w * inv)};
+        *reinterpret_cast<uint2 *>(p.out + row_of(r0 + r) * D + 4 * q) = *reinterpret_cast<const uint2 *>(h);
     };
+    // The warps of this CTA, four values a thread at a time
+    constexpr int Q = D / 4;
     const int w0 = warp - sub;
-    for (int r = gtid >> 4; r < ROWS; r += threads >> 4) {
-        const int d0 = (gtid & 15) * PER;
-        float M = -INFINITY, L = 0.f, acc[PER];
+    float M, L;
+    float4 acc;
+    auto of_warps = [&](int i) {
+        const int r = i / Q;
+        M = -INFINITY, L = 0.f, acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int w = 0; w < warps; w++) M = fmaxf(M, sm_m[w0 + w][r]);
-#pragma unroll
-        for (int i = 0; i < PER; i++) acc[i] = 0.f;
         for (int w = 0; w < warps; w++) {
             const float wgt = weight(sm_m[w0 + w][r], sm_l[w0 + w][r], M);
             L += sm_l[w0 + w][r] * wgt;
-            const float *ow = o_of(w0 + w) + r * PITCH + d0;
-#pragma unroll
-            for (int i = 0; i < PER; i += 4) {
-                const float4 v = *reinterpret_cast<const float4 *>(ow + i);
-                acc[i] += v.x * wgt;
-                acc[i + 1] += v.y * wgt;
-                acc[i + 2] += v.z * wgt;
-                acc[i + 3] += v.w * wgt;
-            }
+            add(acc, *reinterpret_cast<const float4 *>(o_of(w0 + w) + r * PITCH + 4 * (i % Q)), wgt);
         }
-        if (p.nsplit == 1) {
-            store(r, d0, acc, L);
-            continue;
+    };
+    if (p.nsplit == 1) {
+        for (int i = gtid; i < ROWS * Q; i += threads) {
+            of_warps(i);
+            store(i / Q, i % Q, acc, L);
         }
-        const size_t at = (slot + split) * ROWS + r;
-        if ((gtid & 15) == 0) *reinterpret_cast<float2 *>(part_ml + at * 2) = make_float2(M, L);
-#pragma unroll
-        for (int i = 0; i < PER; i += 4)
-            *reinterpret_cast<float4 *>(part_o + at * D + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        return;
     }
-    if (p.nsplit == 1) return;
     // (all four warps of the CTA are this item's from here on)
+    {
+        constexpr int MINE = ROWS * Q / kThreads;
+        float4 mine[MINE];
+        float M_of[MINE], L_of[MINE];
+#pragma unroll
+        for (int k = 0; k < MINE; k++) {
+            of_warps(tid + k * kThreads);
+            mine[k] = acc, M_of[k] = M, L_of[k] = L;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < MINE; k++) {
+            const int i = tid + k * kThreads, r = i / Q;
+            *reinterpret_cast<float4 *>(o_of(0) + r * PITCH + 4 * (i % Q)) = mine[k];
+            if (i % Q == 0) sm_m[0][r] = M_of[k], sm_l[0][r] = L_of[k];
+        }
+    }
+    const int rank = split % p.cluster, per = ROWS / p.cluster;  // this CTA's rows: per * rank ..
+    auto cluster_barrier = [&]() {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    };
+    auto peer = [](const void *at, int of) {
+        uint32_t a;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(of));
+        return a;
+    };
+    cluster_barrier();
+    const int n_clusters = p.nsplit / p.cluster;
+    const size_t slot = (size_t)item * n_clusters + split / p.cluster;
+    float *part_ml = p.partial, *part_o = p.partial + (size_t)kKv8MaxCtas * kKv8MaxRows * 2;
+    for (int i = tid; i < per * Q; i += kThreads) {
+        const int r = per * rank + i / Q, q = i % Q;
+        float m[8], l[8];
+        float4 v[8];
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            m[c] = -INFINITY, l[c] = 0.f, v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c >= p.cluster) continue;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m[c]) : "r"(peer(&sm_m[0][r], c)));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(l[c]) : "r"(peer(&sm_l[0][r], c)));
+            asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                         : "=f"(v[c].x), "=f"(v[c].y), "=f"(v[c].z), "=f"(v[c].w)
+                         : "r"(peer(o_of(0) + r * PITCH + 4 * q, c)));
+        }
+        M = -INFINITY, L = 0.f, acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 8; c++) M = fmaxf(M, m[c]);
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const float wgt = weight(m[c], l[c], M);
+            L += l[c] * wgt;
+            add(acc, v[c], wgt);
+        }
+        if (n_clusters == 1) {
+            store(r, q, acc, L);
+        } else {
+            if (q == 0) *reinterpret_cast<float2 *>(part_ml + (slot * ROWS + r) * 2) = make_float2(M, L);
+            *reinterpret_cast<float4 *>(part_o + (slot * ROWS + r) * D + 4 * q) = acc;
+        }
+    }
+    __syncwarp();
+    cluster_barrier();  // a CTA leaves when its peers have pulled
+    if (n_clusters == 1) return;
     __threadfence();
     __syncthreads();
     if (tid == 0) {
-        int *ticket = p.tickets + item;
-        sm_last = atomicAdd(ticket, 1) == p.nsplit - 1;
+        int *ticket = p.tickets + item * p.cluster + rank;
+        sm_last = atomicAdd(ticket, 1) == n_clusters - 1;
         if (sm_last) *ticket = 0;
     }
     __syncthreads();
     if (!sm_last) return;
     __threadfence();
-    // The last CTA: the splits' (maximum, sum) first, all at once, then O with several loads in flight (a chain of
-    // trips to the L2 otherwise: 74 splits took 16 us of 27).
-    float2 *ml = reinterpret_cast<float2 *>(smem);  // [split][row]
-    for (int i = tid; i < p.nsplit * ROWS; i += kThreads) ml[i] = __ldcg(reinterpret_cast<const float2 *>(part_ml + (slot * ROWS + i) * 2));
-    __syncthreads();
+    // The last cluster, in the clusters' order: eight results in flight (one after the other, 74 of them took 16 us).
+    for (int i = tid; i < per * Q; i += kThreads) {
+        const int r = per * rank + i / Q, q = i % Q;
+        M = -INFINITY, L = 0.f, acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c0 = 0; c0 < n_clusters; c0 += 8) {
+            float2 ml[8];
+            float4 v[8];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int r = 8 * nt + (tid >> 4), t16 = tid & 15, d0 = t16 * PER;
-        float M = -INFINITY, L = 0.f, acc[PER];
-        for (int sp = t16; sp < p.nsplit; sp += 16) M = fmaxf(M, ml[sp * ROWS + r].x);
+            for (int c = 0; c < 8; c++) {
+                ml[c] = make_float2(-INFINITY, 0.f), v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c0 + c >= n_clusters) continue;
+                const size_t at = ((size_t)item * n_clusters + c0 + c) * ROWS + r;
+                ml[c] = __ldcg(reinterpret_cast<const float2 *>(part_ml + at * 2));
+                v[c] = __ldcg(reinterpret_cast<const float4 *>(part_o + at * D + 4 * q));
+            }
+            float M_new = M;
 #pragma unroll
-        for (int d = 1; d < 16; d *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        for (int sp = t16; sp < p.nsplit; sp += 16) {
-            const float2 v = ml[sp * ROWS + r];
-            const float wgt = weight(v.x, v.y, M);
-            L += v.y * wgt;
-            ml[sp * ROWS + r].x = wgt;
-        }
-        // (in the order of a tree over the sixteen threads: the same for every call)
+            for (int c = 0; c < 8; c++) M_new = fmaxf(M_new, ml[c].x);
+            const float old = weight(M, L, M_new);
+            L *= old;
+            acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+            M = M_new;
 #pragma unroll
-        for (int d = 1; d < 16; d *= 2) L += __shfl_xor_sync(0xffffffffu, L, d);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < PER; i++) acc[i] = 0.f;
-        const float *from = part_o + (slot * ROWS + r) * D + d0;
-#pragma unroll 8
-        for (int sp = 0; sp < p.nsplit; sp++) {
-            const float wgt = ml[sp * ROWS + r].x;
-#pragma unroll
-            for (int i = 0; i < PER; i += 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + (size_t)sp * (ROWS * D) + i));
-                acc[i] += v.x * wgt;
-                acc[i + 1] += v.y * wgt;
-                acc[i + 2] += v.z * wgt;
-                acc[i + 3] += v.w * wgt;
+            for (int c = 0; c < 8; c++) {
+                const float wgt = weight(ml[c].x, ml[c].y, M);
+                L += ml[c].y * wgt;
+                add(acc, v[c], wgt);
             }
         }
-        store(r, d0, acc, L);
+        store(r, q, acc, L);
     }
 }
 
 template <int D, int NT>
 int32_t launch(tlc_ctx *ctx, const Params &p) {
     constexpr size_t smem = (size_t)kWarps * stages<D>() * kKv8Block * D;
-    static_assert(smem >= (size_t)kKv8MaxCtas * 8 * NT * sizeof(float2) / 2, "the merge's maxima and sums");
     const dim3 grid((unsigned)(p.nsplit > 1 ? p.items * p.nsplit : (p.items + kWarps / p.warps - 1) / (kWarps / p.warps)));
     static bool configured[64] = {};
     if (!configured[ctx->device & 63]) {
@@ -450,7 +497,26 @@ int32_t launch(tlc_ctx *ctx, const Params &p) {
                                       cudaSharedmemCarveoutMaxShared));
         configured[ctx->device & 63] = true;
     }
-    const cudaError_t le = tlc_launch_pdl(ctx, attention8_kernel<D, NT>, grid, dim3(kThreads), smem, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (p.cluster > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = (unsigned)p.cluster;
+        attr[na].val.clusterDim.y = 1;
+        attr[na++].val.clusterDim.z = 1;
+    }
+    if (ctx->use_pdl && ctx->pdl_small) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    const cudaError_t le = cudaLaunchKernelEx(&cfg, attention8_kernel<D, NT>, p);
     if (le != cudaSuccess) {
         cudaGetLastError();
         return tlc_fail(TLC_ERR_CUDA, "attention8 launch failed: %s", cudaGetErrorString(le));
@@ -459,22 +525,25 @@ int32_t launch(tlc_ctx *ctx, const Params &p) {
     return TLC_OK;
 }
 
-// Warps that share an item of `units` blocks: the fewest microseconds of
+// Warps that share an item of `units` blocks -- 1, 2, 4, or four in each of 2, 4, 8 or a multiple of eight CTAs: the
+// fewest microseconds of
 //   blocks of a warp x (the larger of a block's latency and its share of the HBM, 44 KB/us for the warps of an SM),
-// as often as the SM's eight warps have to be filled, and the merge, in shared memory or through the L2.
+// as often as the SM's eight warps have to be filled, and the merge, in shared memory, in a cluster, or of clusters.
 void share_out(const tlc_ctx *ctx, int D, int units, Params &p) {
     const double latency = D == 64 ? 0.45 : 0.7, share = kKv8Block * D * 2 / 44e3;
     double best = 1e30;
-    for (int w = 1; w <= 4 * kKv8MaxCtas; w = w < 4 ? 2 * w : w + 4) {
-        const int nsplit = w <= kWarps ? 1 : w / kWarps;
-        if (w > 1 && (w > units + 3 || (nsplit > 1 && (p.items > kKv8Tickets || (long long)p.items * nsplit > kKv8MaxCtas || nsplit > kKv8MaxCtas / 2)))) break;
+    for (int w = 1; w <= 4 * kKv8MaxCtas; w = w < 32 ? 2 * w : w + 32) {
+        const int nsplit = w <= kWarps ? 1 : w / kWarps, cluster = nsplit < 8 ? nsplit : 8;
+        if (w > 1 && w >= 2 * units) break;  // (fewer would do)
+        if (nsplit > 8 && ((long long)p.items * nsplit > kKv8MaxCtas || p.items * 8 > kKv8Tickets)) break;
         const long long per_sm = ((long long)p.items * w + ctx->sm_count - 1) / ctx->sm_count, rounds = (per_sm + 7) / 8;
         const double at_once = (double)(per_sm < 8 ? per_sm : 8), block = latency > at_once * share ? latency : at_once * share;
-        const double t = (double)rounds * ((units + w - 1) / w) * block + (w == 1 ? 0.0 : w <= kWarps ? 0.7 : 3.0 + 0.02 * nsplit);
+        const double t = (double)rounds * ((units + w - 1) / w) * block + (w == 1 ? 0.0 : w <= kWarps ? 0.7 : nsplit <= 8 ? 1.5 : 3.5);
         if (t < best) {
             best = t;
             p.warps = w < kWarps ? w : kWarps;
             p.nsplit = nsplit;
+            p.cluster = cluster;
         }
     }
 }
