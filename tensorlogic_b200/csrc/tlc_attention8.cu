@@ -56,8 +56,7 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     return v;
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -169,81 +168,106 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     }
 
     // Softmax of a block's scores s[kg][nt][..] (keys 16 kg + kv8_key(g), .. + kv8_key(g + 8) of rows 2t, 2t + 1): P as
-    // the second product's operand, its sums, and what the rows' O has to be multiplied with.
+    // the second product's operand, this lane's part of its sums, and what the rows' O has to be multiplied with.
     auto softmax = [&](int u, float (&s)[4][NT][4], float factor, uint32_t (&pf)[4][NT][2], float (&psum)[NT][2], float (&corr)[NT][2]) {
         const bool masked = (u + 1) * kKv8Block > all_see;
+        float shift[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            float mx[2] = {-INFINITY, -INFINITY};
+            float mx[2][4];
 #pragma unroll
-            for (int kg = 0; kg < 4; kg++)
+            for (int kg = 0; kg < 4; kg++) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float x = s[kg][nt][e] * factor;
-                    if (masked && u * kKv8Block + 16 * kg + 4 * (g >> 1) + (g & 1) + 2 * (e >> 1) >= end[nt][e & 1]) x = -INFINITY;
-                    s[kg][nt][e] = x;
-                    mx[e & 1] = fmaxf(mx[e & 1], x);
+                    s[kg][nt][e] *= factor;
+                    if (masked && u * kKv8Block + 16 * kg + 4 * (g >> 1) + (g & 1) + 2 * (e >> 1) >= end[nt][e & 1]) s[kg][nt][e] = -INFINITY;
                 }
-            float shift[2];
+                mx[0][kg] = fmaxf(s[kg][nt][0], s[kg][nt][2]);
+                mx[1][kg] = fmaxf(s[kg][nt][1], s[kg][nt][3]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) shift[nt][e] = fmaxf(fmaxf(mx[e][0], mx[e][1]), fmaxf(mx[e][2], mx[e][3]));
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) shift[nt][e] = fmaxf(shift[nt][e], __shfl_xor_sync(0xffffffffu, shift[nt][e], d));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-#pragma unroll
-                for (int d = 4; d < 32; d *= 2) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
-                const float m_new = fmaxf(m_run[nt][e], mx[e]), m_safe = m_new == -INFINITY ? 0.f : m_new;
+                const float m_new = fmaxf(m_run[nt][e], shift[nt][e]), m_safe = m_new == -INFINITY ? 0.f : m_new;
                 corr[nt][e] = exp2_of(m_run[nt][e] - m_safe);
                 m_run[nt][e] = m_new;
-                shift[e] = kShift - m_safe;
+                shift[nt][e] = kShift - m_safe;
                 psum[nt][e] = 0.f;
             }
 #pragma unroll
             for (int kg = 0; kg < 4; kg++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const __half2 v = __floats2half2_rn(exp2_of(s[kg][nt][2 * h] + shift[0]), exp2_of(s[kg][nt][2 * h + 1] + shift[1]));
+                    const __half2 v = __floats2half2_rn(exp2_of(s[kg][nt][2 * h] + shift[nt][0]), exp2_of(s[kg][nt][2 * h + 1] + shift[nt][1]));
                     psum[nt][0] += __low2float(v);
                     psum[nt][1] += __high2float(v);
                     pf[kg][nt][h] = turned(*reinterpret_cast<const uint32_t *>(&v));
                 }
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-#pragma unroll
-                for (int d = 4; d < 32; d *= 2) psum[nt][e] += __shfl_xor_sync(0xffffffffu, psum[nt][e], d);
-                l_run[nt][e] = l_run[nt][e] * corr[nt][e] + psum[nt][e];
-            }
         }
     };
-    // O of 16 values of d (index dt): times corr, plus the block's product
-    auto join = [&](int dt, int nt, const float (&acc)[4], float factor, const float (&corr)[NT][2]) {
+    // The rows' sums of P over the lanes, while the second product runs.
+    auto reduce = [&](float (&psum)[NT][2], const float (&corr)[NT][2]) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[nt][dt][e] = o[nt][dt][e] * corr[nt][e & 1] + acc[e] * factor;
+        for (int d = 4; d < 32; d *= 2)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) psum[nt][e] += __shfl_xor_sync(0xffffffffu, psum[nt][e], d);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) l_run[nt][e] = l_run[nt][e] * corr[nt][e] + psum[nt][e];
+    };
+    // O of 16 values of d (index dt): times corr, plus the block's product less 128 times the sum of P where V is codes
+    auto join = [&](int dt, int nt, const float (&acc)[4], float factor, const float (&less)[NT][2], const float (&corr)[NT][2]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[nt][dt][e] = fmaf(o[nt][dt][e], corr[nt][e & 1], (acc[e] - less[nt][e & 1]) * factor);
     };
 
+    // (Products that follow each other belong to different sums: a warp issues in order, and a sum is a chain.)
+    constexpr int WIDE = NT == 1 ? 2 : 1;  // pairs of 16 values of d whose second products run side by side
     int step = 0;
     float2 factor = first;
     for (int u = u0; u < n_sealed; u += stride) {
         const float sk = factor.x, sv = factor.y;
         if (u + stride < n_sealed) factor = scales[u + stride];  // the next block's, a trip to memory ahead
-        float s[4][NT][4], psum[NT][2], corr[NT][2];
+        float s[4][NT][4], psum[NT][2], corr[NT][2], less[NT][2];
         uint32_t pf[4][NT][2];
         fetch(step + ST - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
         uint32_t at = ring + (uint32_t)(step % ST * STAGE);
 #pragma unroll
-        for (int kg = 0; kg < 4; kg++) {
+        for (int kg = 0; kg < 4; kg++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 s[kg][nt][0] = s[kg][nt][2] = start[nt][0];
                 s[kg][nt][1] = s[kg][nt][3] = start[nt][1];
             }
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) {
-                const uint4 w = lds128(at + (uint32_t)((kg * (D / 32) + c) * 512));
+        for (int c = 0; c < D / 32; c++) {
+            uint4 w[4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    mma(s[kg][nt], low2(w.x), low2(w.z), high2(w.x), high2(w.z), qf[nt][2 * c][0], qf[nt][2 * c][1]);
-                    mma(s[kg][nt], low2(w.y), low2(w.w), high2(w.y), high2(w.w), qf[nt][2 * c + 1][0], qf[nt][2 * c + 1][1]);
-                }
-            }
+            for (int kg = 0; kg < 4; kg++) w[kg] = lds128(at + (uint32_t)((kg * (D / 32) + c) * 512));
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    mma(s[kg][nt], low2(w[kg].x), low2(w[kg].z), high2(w[kg].x), high2(w[kg].z), qf[nt][2 * c][0], qf[nt][2 * c][1]);
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    mma(s[kg][nt], low2(w[kg].y), low2(w[kg].w), high2(w[kg].y), high2(w[kg].w), qf[nt][2 * c + 1][0], qf[nt][2 * c + 1][1]);
         }
         step++;
         softmax(u, s, kUp * sk * p.scale * kLog2e, pf, psum, corr);
@@ -251,26 +275,40 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
         at = ring + (uint32_t)(step % ST * STAGE);
 #pragma unroll
-        for (int c = 0; c < D / 32; c++) {
-            float acc[2][NT][4];
+        for (int c0 = 0; c0 < D / 32; c0 += WIDE) {
+            float acc[WIDE][2][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int c = 0; c < WIDE; c++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[0][nt][e] = acc[1][nt][e] = psum[nt][e & 1] * (-128.f / kUp);
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[c][0][nt][e] = acc[c][1][nt][e] = 0.f;
 #pragma unroll
             for (int kg = 0; kg < 4; kg++) {
-                const uint4 w = lds128(at + (uint32_t)((kg * (D / 32) + c) * 512));
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    mma(acc[0][nt], low2(w.x), low2(w.y), high2(w.x), high2(w.y), pf[kg][nt][0], pf[kg][nt][1]);
-                    mma(acc[1][nt], low2(w.z), low2(w.w), high2(w.z), high2(w.w), pf[kg][nt][0], pf[kg][nt][1]);
+                for (int c = 0; c < WIDE; c++) {
+                    const uint4 w = lds128(at + (uint32_t)((kg * (D / 32) + c0 + c) * 512));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        mma(acc[c][0][nt], low2(w.x), low2(w.y), high2(w.x), high2(w.y), pf[kg][nt][0], pf[kg][nt][1]);
+                        mma(acc[c][1][nt], low2(w.z), low2(w.w), high2(w.z), high2(w.w), pf[kg][nt][0], pf[kg][nt][1]);
+                    }
                 }
             }
+            if (c0 == 0) {
+                reduce(psum, corr);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                join(2 * c, nt, acc[0][nt], kUp * sv, corr);
-                join(2 * c + 1, nt, acc[1][nt], kUp * sv, corr);
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) less[nt][e] = psum[nt][e] * (128.f / kUp);
             }
+#pragma unroll
+            for (int c = 0; c < WIDE; c++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    join(2 * (c0 + c), nt, acc[c][0][nt], kUp * sv, less, corr);
+                    join(2 * (c0 + c) + 1, nt, acc[c][1][nt], kUp * sv, less, corr);
+                }
         }
         step++;
     }
@@ -278,32 +316,38 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     if (units > sealed && sealed % stride == u0) {
         const uint4 *kt = reinterpret_cast<const uint4 *>(p.c.open + head * (2 * STAGE)) + lane, *vt = kt + STAGE / 8;
         float s[4][NT][4], psum[NT][2], corr[NT][2];
+        const float none[NT][2] = {};
         uint32_t pf[4][NT][2];
 #pragma unroll
-        for (int kg = 0; kg < 4; kg++) {
+        for (int kg = 0; kg < 4; kg++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[kg][nt][0] = s[kg][nt][1] = s[kg][nt][2] = s[kg][nt][3] = 0.f;
 #pragma unroll
-            for (int k16 = 0; k16 < D / 16; k16++) {
-                const uint4 w = kt[(kg * (D / 16) + k16) * 32];
+        for (int k16 = 0; k16 < D / 16; k16++) {
+            uint4 w[4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) mma(s[kg][nt], w.x, w.z, w.y, w.w, qf[nt][k16][0], qf[nt][k16][1]);
-            }
+            for (int kg = 0; kg < 4; kg++) w[kg] = kt[(kg * (D / 16) + k16) * 32];
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma(s[kg][nt], w[kg].x, w[kg].z, w[kg].y, w[kg].w, qf[nt][k16][0], qf[nt][k16][1]);
         }
         softmax(sealed, s, p.scale * kLog2e, pf, psum, corr);
+        reduce(psum, corr);
 #pragma unroll
         for (int dt = 0; dt < D / 16; dt++) {
             float acc[NT][4];
+            uint4 w[4];
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++) w[kg] = vt[(kg * (D / 16) + dt) * 32];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
-            for (int kg = 0; kg < 4; kg++) {
-                const uint4 w = vt[(kg * (D / 16) + dt) * 32];
+            for (int kg = 0; kg < 4; kg++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) mma(acc[nt], w.x, w.z, w.y, w.w, pf[kg][nt][0], pf[kg][nt][1]);
-            }
+                for (int nt = 0; nt < NT; nt++) mma(acc[nt], w[kg].x, w[kg].z, w[kg].y, w[kg].w, pf[kg][nt][0], pf[kg][nt][1]);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) join(dt, nt, acc[nt], 1.f, corr);
+            for (int nt = 0; nt < NT; nt++) join(dt, nt, acc[nt], 1.f, none, corr);
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
