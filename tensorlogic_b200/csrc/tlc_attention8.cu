@@ -82,7 +82,8 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     tlc_pdl_after_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int warps = p.warps, sub = warp % warps, gtid = sub * 32 + lane, threads = 32 * warps;
-    const int item = p.nsplit > 1 ? blockIdx.x / p.nsplit : blockIdx.x * (kWarps / warps) + warp / warps;
+    // (neighbours in different CTAs: a batch in the order of its lengths leaves no SM the longest ones)
+    const int item = p.nsplit > 1 ? blockIdx.x / p.nsplit : blockIdx.x + warp / warps * gridDim.x;
     if (item >= p.items) return;
     const int split = p.nsplit > 1 ? blockIdx.x % p.nsplit : 0;
     const int rt = item % p.row_tiles, hk = item / p.row_tiles % p.c.n_kv_heads, b = item / p.row_tiles / p.c.n_kv_heads;
@@ -533,7 +534,13 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
 template <int D, int NT>
 int32_t launch(tlc_ctx *ctx, const Params &p) {
     constexpr size_t smem = (size_t)kWarps * stages<D>() * kKv8Block * D;
-    const dim3 grid((unsigned)(p.nsplit > 1 ? p.items * p.nsplit : (p.items + kWarps / p.warps - 1) / (kWarps / p.warps)));
+    int ctas = p.items * p.nsplit;
+    if (p.nsplit == 1) {  // both places of every SM, as far as items go
+        const int groups = kWarps / p.warps, least = (p.items + groups - 1) / groups;
+        ctas = p.items < 2 * ctx->sm_count ? p.items : 2 * ctx->sm_count;
+        if (ctas < least) ctas = least;
+    }
+    const dim3 grid((unsigned)ctas);
     static bool configured[64] = {};
     if (!configured[ctx->device & 63]) {
         TLC_CUDA(cudaFuncSetAttribute(attention8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
