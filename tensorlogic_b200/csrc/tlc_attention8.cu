@@ -24,7 +24,6 @@
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kTcRows = 1024;  // (query, head) rows of a KV head from which a prompt runs on tcgen05
 constexpr float kShift = 12.f;        // P is held times 2^12
 constexpr float kUp = 16777216.f;     // the codes' 2^24
 constexpr float kLog2e = 1.4426950408889634f;
@@ -578,10 +577,12 @@ int32_t launch(tlc_ctx *ctx, const Params &p) {
 
 // Warps that share an item of `units` blocks -- 1, 2, 4, or four in each of 2, 4, 8 or a multiple of eight CTAs: the
 // fewest microseconds of
-//   blocks of a warp x (the larger of a block's latency and its share of the HBM, 44 KB/us for the warps of an SM),
+//   blocks of a warp x (the larger of a block's latency and its share of the SM, 44 KB/us for its warps),
 // as often as the SM's eight warps have to be filled, and the merge, in shared memory, in a cluster, or of clusters.
-void share_out(const tlc_ctx *ctx, int D, int units, Params &p) {
-    const double latency = D == 64 ? 0.45 : 0.7, share = kKv8Block * D * 2 / 44e3;
+// Sixteen queries behind 1000 positions, 32 heads of 128: one warp 28.5 us, two 19.8, four 12.8, sixteen 11.8; 192
+// queries: 49.2, 31.9, 35.6, 68.
+double share_out(const tlc_ctx *ctx, int D, int nt, int units, Params &p) {
+    const double latency = D == 64 ? nt == 1 ? 0.85 : 1.05 : nt == 1 ? 1.2 : 1.6, share = kKv8Block * D * 2 / 44e3;
     double best = 1e30;
     for (int w = 1; w <= 4 * kKv8MaxCtas; w = w < 32 ? 2 * w : w + 32) {
         const int nsplit = w <= kWarps ? 1 : w / kWarps, cluster = nsplit < 8 ? nsplit : 8;
@@ -597,6 +598,17 @@ void share_out(const tlc_ctx *ctx, int D, int units, Params &p) {
             p.cluster = cluster;
         }
     }
+    return best;
+}
+// Microseconds that the tcgen05 form takes more than a launch of the other one: another launch and the longer start of its
+// CTAs, the image of the blocks (three bytes moved a value), and its tiles of 128 rows x 64 keys, by the longest CTA or by
+// what an SM gets through.  32 heads of 128: 192 queries 12.1 us here, 8.6 there, behind 1000 positions 31.9 and 23.5;
+// 64 behind 1000 15.2 and 24.5.  2048 queries 225 and 51.
+double tcgen05_us(const tlc_ctx *ctx, int D, int Hkv, int G, int I, int pos0) {
+    const int rq = 128 / G, tiles = (I + rq - 1) / rq, units = (pos0 + I + kKv8Block - 1) / kKv8Block;
+    const double image = (double)units * Hkv * kKv8Block * D * 6 / 5e6, longest = units * (D == 64 ? 0.45 : 0.55);
+    const double all = (double)tiles * Hkv * (pos0 + 0.5 * I + kKv8Block) / kKv8Block / ctx->sm_count * (D == 64 ? 0.45 : 0.7);
+    return 2.0 + image + (longest > all ? longest : all);
 }
 
 }  // namespace
@@ -623,16 +635,6 @@ extern "C" int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
     const int G = n_heads / Hkv;
     TLC_REQUIRE(batch <= 65535 && (long long)n_queries * G <= INT_MAX / 64, TLC_ERR_INVALID_DIMENSION,
                 "attention8: %d sequences of %d queries", batch, n_queries);
-    // Long prompts: on tcgen05, a sequence at a time.
-    if (!positions_dev && (long long)n_queries * G >= kTcRows && G <= 128) {
-        for (int b = 0; b < batch; b++) {
-            const size_t at = (size_t)b * n_queries * n_heads * D;
-            if (int32_t rc = kv8_attention_tc(ctx, cache, layer, sequence + b, static_cast<const __half *>(q_dev) + at,
-                                              static_cast<__half *>(out_dev) + at, n_queries, n_heads, q_pos0, scale))
-                return rc;
-        }
-        return TLC_OK;
-    }
     Params p{};
     p.q = static_cast<const __half *>(q_dev);
     p.out = static_cast<__half *>(out_dev);
@@ -652,7 +654,16 @@ extern "C" int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
     const long long items = (long long)batch * Hkv * p.row_tiles;
     TLC_REQUIRE(items <= INT_MAX, TLC_ERR_INVALID_DIMENSION, "attention8: %d sequences of %d queries", batch, n_queries);
     p.items = (int)items;
-    share_out(ctx, D, (int)((T + kKv8Block - 1) / kKv8Block), p);
+    const double t = share_out(ctx, D, nt, (int)((T + kKv8Block - 1) / kKv8Block), p);
+    if (n_queries > 1 && G <= 128 && batch * tcgen05_us(ctx, D, Hkv, G, n_queries, q_pos0) < t) {  // (a sequence at a time)
+        for (int b = 0; b < batch; b++) {
+            const size_t at = (size_t)b * n_queries * n_heads * D;
+            if (int32_t rc = kv8_attention_tc(ctx, cache, layer, sequence + b, static_cast<const __half *>(q_dev) + at,
+                                              static_cast<__half *>(out_dev) + at, n_queries, n_heads, q_pos0, scale))
+                return rc;
+        }
+        return TLC_OK;
+    }
     if (D == 64) return nt == 1 ? launch<64, 1>(ctx, p) : launch<64, 2>(ctx, p);
     return nt == 1 ? launch<128, 1>(ctx, p) : launch<128, 2>(ctx, p);
 }
