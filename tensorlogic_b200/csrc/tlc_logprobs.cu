@@ -443,7 +443,9 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
         }
         __syncthreads();
         {
-            const unsigned long long least = bound;  // 0: fewer than k groups have anything
+            // 0: fewer than k groups have anything.  The k-th best of the slices before (0: there are not so many) bounds
+            // as well: it keeps the last, short slice, where few groups have anything, from being ranked whole.
+            const unsigned long long so_far = best[0][p.top - 1], least = bound > so_far ? bound : so_far;
             // (a thread whose maximum is below the bound's value has nothing to add)
             const __half least_x = least ? value_of(least) : __ushort_as_half((unsigned short)0xFBFF);  // the lowest f16
             if (mine >= __half2float(least_x)) {

@@ -169,3 +169,16 @@ def test_refusals(dev):
     with pytest.raises(TensorError):
         token_logprobs(x, [0, 1], top_k=33)
     dev.synchronize()
+
+
+@pytest.mark.parametrize("vocab", [131600, 8 * 16384 + 8 * 8 * 31, 140001])
+def test_short_last_slice(dev, vocab):
+    """Slices that end with a few pieces: the best logits before them, in them, and everywhere."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((4, vocab)).astype(np.float16)
+    x[1] = np.arange(vocab) * (50.0 / vocab)
+    x[2] = np.arange(vocab)[::-1] * (50.0 / vocab)
+    x[3] = 1
+    for top in (1, 32):
+        check(dev, x, rng.integers(0, vocab, 4), top)
+    dev.synchronize()
