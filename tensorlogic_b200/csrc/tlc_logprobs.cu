@@ -518,6 +518,34 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     });
 }
 
+// How many 16-byte pieces a slice has, at most.
+constexpr long long slice_pieces(int vocab, int ctas) { return ((long long)vocab + 14) / 8 / ctas + 1; }
+
+// CTAs a row, by cost in microseconds as fitted to calls of 1 to 400 rows of 16000 to 151936 logits with 1, 2, 4 and 8
+// CTAs a row.  A row costs the joining of its CTAs and a CTA's work: a turn of 2048 pieces with alternatives (4.4, a
+// slice held in 1 or 2 pieces a thread 3.05 or 3.5), 15000 logits a microsecond without.  As many clusters as find an SM
+// for each CTA run at once (4 or 8 CTAs must lie in one part of the chip: a fifth of the SMs stays empty); further ones
+// share SMs and cost 0.85 of that.  37 x 32000 with alternatives takes 8.6 us with 2 CTAs a row, 9.8 with 4 and 14.7
+// with 8; 37 x 100003 21.7, 18.1 and 18.5; 148 x 100003 32.4, 43.9 and 51.2.
+int ctas_a_row(int sms, int rows, int vocab, bool alternatives) {
+    constexpr double kJoin[2][4] = {{0, 1.1, 1.3, 2.1}, {0, 0.6, 0.7, 1.6}};
+    int best = 1;
+    double least = 1e30;
+    for (int c = 1, i = 0; c <= kMaxCluster; c *= 2, i++) {
+        const long long n = slice_pieces(vocab, c), held = n <= kTopThreads ? 1 : n <= 2 * kTopThreads ? 2 : 4;
+        const double work = alternatives ? (double)((n + held * kTopThreads - 1) / (held * kTopThreads)) * (2.6 + 0.45 * held) : n * 8 / 15000.0;
+        int at_once = (c <= 2 ? sms : sms * 4 / 5) / c;
+        if (at_once < 1) at_once = 1;
+        const int layers = (rows - 1) / at_once + 1;
+        const double cost = kJoin[alternatives][i] + work * (layers == 1 ? 1 : 0.85 * layers);
+        if (cost < least) {
+            least = cost;
+            best = c;
+        }
+    }
+    return best;
+}
+
 template <int PIECES>
 cudaError_t launch_top(tlc_ctx *ctx, cudaLaunchConfig_t &cfg, const LogprobParams &p) {
     constexpr size_t smem = list_size<PIECES>() * sizeof(unsigned long long);
@@ -557,10 +585,7 @@ extern "C" int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int3
     p.vocab = vocab;
     p.top = top_k;
     p.status = ctx->dev_status;
-    // CTAs a row: more of them while SMs have room and slices are long; with alternatives, where a slice of more than 32
-    // values a thread costs its CTA the second place on the SM, until slices are that short.
-    int c = 1;
-    while (c < kMaxCluster && (((long long)rows * c <= ctx->sm_count && vocab / c >= 4096) || (top_k > 0 && vocab / c > kTopThreads * 32))) c *= 2;
+    const int c = ctas_a_row(ctx->sm_count, rows, vocab, top_k > 0);
     p.cluster = c;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * c));
@@ -580,10 +605,10 @@ extern "C" int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int3
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    const long long values = ((long long)vocab + 14) / 8 / c + 1;  // 16-byte pieces of a slice, at most
+    const long long pieces = slice_pieces(vocab, c);
     const cudaError_t le = top_k == 0                  ? cudaLaunchKernelEx(&cfg, logprob_kernel, p)
-                           : values <= kTopThreads     ? launch_top<1>(ctx, cfg, p)
-                           : values <= 2 * kTopThreads ? launch_top<2>(ctx, cfg, p)
+                           : pieces <= kTopThreads     ? launch_top<1>(ctx, cfg, p)
+                           : pieces <= 2 * kTopThreads ? launch_top<2>(ctx, cfg, p)
                                                        : launch_top<4>(ctx, cfg, p);
     if (le != cudaSuccess) {
         cudaGetLastError();
