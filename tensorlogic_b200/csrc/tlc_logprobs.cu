@@ -6,10 +6,10 @@
 // keeps a running s = sum 2^y, t = sum 2^y y with y = x log2(e) + c, one fused multiply-add, and c = -m log2(e) in f32
 // for the largest x so far: whatever c is rounded to, log2 p(x) = y - log2 s, so that large logits lose nothing.
 //
-// Alternatives (logprob_top_kernel): the slice is held in registers, 8 to 64 values a thread, and taken once more for
-// them.  (value, lowest id first) is one 48-bit key per logit, so no two are equal.  The k-th largest of the best keys
-// of 128 groups of four threads is a bound that at least k logits reach, and none but those of at most k groups can:
-// these few are collected and ranked by counting.
+// Alternatives (logprob_top_kernel): the slice is taken in turns of at most 16384 logits, held in registers, 8 to 32 a
+// thread, and looked at once more for them.  (value, earliest first) is one key per logit, so no two are equal.  The k-th
+// largest of the best keys of 64 groups of eight threads is a bound that at least k logits reach, and none but those of
+// at most k groups can: these few are collected and ranked by counting.
 #include <cuda_fp16.h>
 
 #include "tlc_internal.h"
@@ -19,10 +19,10 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kUnroll = 4;  // 16-byte pieces of a thread in flight, twice
 constexpr float kLow = -60000.f;  // 2^y of the lowest f16 is zero beside any value from here on
-constexpr int kTopThreads = 512, kTopWarps = kTopThreads / 32, kGroups = kTopThreads / 4;
+constexpr int kTopThreads = 512, kTopWarps = kTopThreads / 32, kGroups = 64;
 constexpr int kMaxTop = 32, kMaxCluster = 8;
-// what k groups of threads with so many 16-byte pieces each hold, and the best of earlier passes
-template <int PIECES> constexpr int list_size() { return kMaxTop * PIECES * 8 * 4 + kMaxTop; }
+// what k groups of threads with so many 16-byte pieces each hold
+template <int PIECES> constexpr int list_size() { return kMaxTop * (kTopThreads / kGroups) * PIECES * 8; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_of(float x) {
@@ -283,44 +283,31 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
     if (tid == 0) store_row(p, row, target, run);
 }
 
-// Larger for a larger value, then for a smaller id; 0: no logit.
-__device__ __forceinline__ unsigned long long key_of(__half x, unsigned id) {
+// Alternatives are compared by keys: larger for a larger value, then for an earlier one, 0 for no logit.  Within a turn
+// (of at most 16384 logits) value << 16 | 0xFFFF - place, in a row value << 32 | 0xFFFFFFFF - id.
+__device__ __forceinline__ unsigned value_key(__half x) {
     const unsigned short b = __half_as_ushort(x);
-    const unsigned v = (b & 0x8000) ? (unsigned short)~b : (unsigned short)(b | 0x8000);
-    return (unsigned long long)v << 32 | (0xFFFFFFFFu - id);
+    return (b & 0x8000) ? (unsigned short)~b : (unsigned short)(b | 0x8000);
 }
-__device__ __forceinline__ __half value_of(unsigned long long key) {
-    const unsigned short v = (unsigned short)(key >> 32);
+__device__ __forceinline__ __half value_of(unsigned v) {
     return __ushort_as_half((v & 0x8000) ? (unsigned short)(v & 0x7FFF) : (unsigned short)~v);
-}
-
-// take(key, its index, how many are larger) for those of n keys (not 0) that fewer than `top` are larger than: up to 32
-// threads a key.
-template <typename F>
-__device__ __forceinline__ void ranked(const unsigned long long *keys, int n, int top, F &&take) {
-    int lanes = 32;
-    while (lanes > 1 && lanes * n > kTopThreads) lanes >>= 1;
-    const int sub = threadIdx.x & (lanes - 1), step = kTopThreads / lanes;
-    for (int i0 = 0; i0 < n; i0 += step) {
-        const int i = i0 + threadIdx.x / lanes;
-        const unsigned long long key = i < n ? keys[i] : 0;
-        int above = 0;
-        for (int j = sub; j < n; j += lanes) above += keys[j] > key;
-        for (int o = 1; o < lanes; o *= 2) above += __shfl_xor_sync(0xffffffffu, above, o);
-        if (sub == 0 && key > 0 && above < top) take(key, i, above);
-    }
 }
 
 // With alternatives.
 template <int PIECES>
 __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const LogprobParams p) {
-    extern __shared__ __align__(16) unsigned long long list[];  // [list_size<PIECES>()]
-    __shared__ __align__(16) unsigned long long group_best[kGroups];
-    __shared__ unsigned long long best[kMaxCluster][kMaxTop];  // of this CTA's slices; in the first CTA, of all
-    __shared__ Sums sums[kMaxCluster];
-    __shared__ float warp_max[kTopWarps], warp_s[kTopWarps], warp_t[kTopWarps];
-    __shared__ unsigned long long bound;
-    __shared__ int n_list;
+    constexpr int kTurn = kTopThreads * PIECES;  // pieces
+    extern __shared__ __align__(16) unsigned list[];  // [list_size<PIECES>()]
+    __shared__ __align__(16) unsigned group_best[kGroups];
+    __shared__ __align__(16) unsigned long long best[kMaxCluster][kMaxTop];  // of this CTA's turns; in the first CTA, of all
+    __shared__ __align__(16) unsigned turn_best[kMaxTop];
+    __shared__ __align__(16) Sums sums[kMaxCluster];
+    __shared__ __align__(16) float warp_max[kTopWarps], warp_s[kTopWarps], warp_t[kTopWarps];
+    struct Found {
+        unsigned bound;
+        int n;
+    };
+    __shared__ __align__(16) Found found;
     if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     tlc_pdl_after_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -330,41 +317,53 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     if (tid == 0 && rank == 0) target = target_of(p, row);
     // The row in 16-byte pieces of memory: the first and the last may reach into other rows, and past the array.
     const int ahead = (int)(((uintptr_t)x0 & 15) >> 1);  // values of the first piece in front of the row
-    const __half *base = x0 - ahead, *lo = p.logits, *hi = p.logits + (size_t)p.rows * p.vocab;
+    const __half *base = x0 - ahead;
     const long long pieces = ((long long)ahead + p.vocab + 7) / 8, share = (pieces + p.cluster - 1) / p.cluster;
     const long long first = rank * share, end = first + share < pieces ? first + share : pieces;
 
     if (tid < p.top) best[0][tid] = 0;
+    if (tid < kGroups) group_best[tid] = 0;
     Sums run = {INFINITY, 0.f, 0.f};
-    const __half2 neg_inf = __float2half2_rn(-INFINITY), neg_zero = __floats2half2_rn(-0.f, -0.f);
-    for (long long p0 = first; p0 < end; p0 += kTopThreads * PIECES) {
+    for (long long p0 = first; p0 < end; p0 += kTurn) {
         __half2 v[PIECES * 4];
+        {
+            uint4 w[PIECES];
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const long long at = p0 + tid + i * kTopThreads;
-            const __half *src = base + at * 8;
-            uint4 w = make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);  // -inf
-            if (at < end) {
-                if (src >= lo && src + 8 <= hi) {
-                    w = *reinterpret_cast<const uint4 *>(src);
-                } else {
-                    __half *h = reinterpret_cast<__half *>(&w);
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (src + e >= lo && src + e < hi) h[e] = src[e];
-                }
-                if (at == 0 || at + 1 == pieces) {  // not this row's
-                    unsigned short *h = reinterpret_cast<unsigned short *>(&w);
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (at * 8 + e < ahead || at * 8 + e >= (long long)ahead + p.vocab) h[e] = 0xFC00;
-                }
+            for (int i = 0; i < PIECES; i++) {
+                const long long at = p0 + tid + i * kTopThreads;
+                w[i] = make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);  // -inf
+                if (at > 0 && at + 1 < pieces && at < end) w[i] = *reinterpret_cast<const uint4 *>(base + at * 8);
             }
-            const __half2 *h = reinterpret_cast<const __half2 *>(&w);
-            // x * -0 + x is NaN for what is not finite, x for the rest (+0 for -0); the maximum passes over NaN
+            // the row's first and last piece, value by value
+#pragma unroll 1
+            for (int side = 0; side < 2; side++) {
+                const long long at = side ? pieces - 1 : 0, off = at - p0 - tid;
+                if (at >= end || off < 0 || off >= kTurn || (off & (kTopThreads - 1))) continue;
+                unsigned long long low = 0, high = 0;
+#pragma unroll 1
+                for (int e = 0; e < 8; e++) {
+                    const long long n = at * 8 + e - ahead;
+                    const unsigned long long x = n >= 0 && n < p.vocab ? __half_as_ushort(x0[n]) : 0xFC00;
+                    low = low >> 16 | high << 48;
+                    high = high >> 16 | x << 48;
+                }
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[4 * i + e] = __hmax2(__hfma2(h[e], neg_zero, h[e]), neg_inf);
+                for (int i = 0; i < PIECES; i++)
+                    if (off == i * kTopThreads) w[i] = make_uint4((unsigned)low, (unsigned)(low >> 32), (unsigned)high, (unsigned)(high >> 32));
+            }
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) clean(w[i], __float2half2_rn(-INFINITY), *reinterpret_cast<__half2(*)[4]>(&v[4 * i]));
         }
+        // the key of a turn's value: 8 places a piece
+        auto key_of = [&](__half x, int e, int half) { return value_key(x) << 16 | (0xFFFF - (unsigned)((tid + (e >> 2) * kTopThreads) * 8 + 2 * (e & 3) + half)); };
+        // of the values that `hit` says, one bit each (e, and 16 + e for the upper half), those of value e
+        auto value_at = [&](int e, int half) {
+            __half2 x = v[0];
+#pragma unroll
+            for (int i = 1; i < PIECES * 4; i++)
+                if (e == i) x = v[i];
+            return half ? __high2half(x) : __low2half(x);
+        };
         __half2 mx = v[0];
 #pragma unroll
         for (int e = 1; e < PIECES * 4; e++) mx = __hmax2(mx, v[e]);
@@ -372,47 +371,36 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
         float m = mine;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        __syncthreads();  // (what the slice before left here has been read)
+        __syncthreads();  // (what the turn before left here has been read)
         if (lane == 0) warp_max[warp] = m;
-        {
-            // this group's best key: of the values equal to a thread's maximum, the first
-            unsigned long long k = 0;
-            if (mine > -INFINITY) {
-                const __half want = __float2half_rn(mine);
-                unsigned id = 0;
+        if (mine > -INFINITY) {
+            // the first of the values equal to the thread's maximum
+            const __half2 want = __float2half2_rn(mine);
+            unsigned hit = 0;
 #pragma unroll
-                for (int e = PIECES * 4 - 1; e >= 0; e--) {
-                    const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kTopThreads) * 8 + 2 * (e & 3) - ahead);
-                    if (__heq(__high2half(v[e]), want)) id = at + 1;
-                    if (__heq(__low2half(v[e]), want)) id = at;
-                }
-                k = key_of(want, id);
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o *= 2) {
-                const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
-                k = other > k ? other : k;
-            }
-            if ((tid & 3) == 0) group_best[tid >> 2] = k;
-            if (tid == 0) {
-                bound = 0;
-                n_list = p.top;
-            }
+            for (int e = 0; e < PIECES * 4; e++) hit |= __heq2_mask(v[e], want) & (0x10001u << e);
+            const int e = __ffs((hit | hit >> 16) & 0xFFFFu) - 1, half = hit >> e & 1 ? 0 : 1;
+            atomicMax(&group_best[tid & (kGroups - 1)], key_of(__low2half(want), e, half));
         }
+        if (tid == 0) found = {0, 0};
+        if (tid < p.top) turn_best[tid] = 0;
         __syncthreads();
         m = warp_max[0];
 #pragma unroll
         for (int w = 1; w < kTopWarps; w++) m = fmaxf(m, warp_max[w]);
         {
-            // group tid / 4, against a quarter of the others: the one with k - 1 better ones is the bound
-            const unsigned long long own = group_best[tid >> 2];
+            // group tid / 8, against an eighth of the others: the one with k - 1 better ones is the bound
+            const unsigned own = group_best[tid >> 3];
+            const uint4 *all = reinterpret_cast<const uint4 *>(group_best);
             int better = 0;
-#pragma unroll 8
-            for (int i = 0; i < kGroups / 4; i++) better += group_best[4 * i + (tid & 3)] > own;
-            better += __shfl_xor_sync(0xffffffffu, better, 1);
-            better += __shfl_xor_sync(0xffffffffu, better, 2);
-            if ((tid & 3) == 0 && better == p.top - 1 && own > 0) bound = own;
-            if (tid < p.top) list[tid] = best[0][tid];
+#pragma unroll
+            for (int i = 0; i < kGroups / 32; i++) {
+                const uint4 g = all[8 * i + (tid & 7)];
+                better += (g.x > own) + (g.y > own) + (g.z > own) + (g.w > own);
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o *= 2) better += __shfl_xor_sync(0xffffffffu, better, o);
+            if ((tid & 7) == 0 && better == p.top - 1 && own > 0) found.bound = own;
         }
         float s = 0.f, t = 0.f;
         const float c = -(m * kLog2e);
@@ -442,22 +430,25 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
             warp_t[warp] = t;
         }
         __syncthreads();
+        if (tid < kGroups) group_best[tid] = 0;  // for the next turn
         {
-            // 0: fewer than k groups have anything.  The k-th best of the slices before (0: there are not so many) bounds
-            // as well: it keeps the last, short slice, where few groups have anything, from being ranked whole.
-            const unsigned long long so_far = best[0][p.top - 1], least = bound > so_far ? bound : so_far;
-            // (a thread whose maximum is below the bound's value has nothing to add)
-            const __half least_x = least ? value_of(least) : __ushort_as_half((unsigned short)0xFBFF);  // the lowest f16
+            // 0: fewer than k groups have anything.  The k-th best of the turns before (0: there are not so many) bounds
+            // as well: it keeps the last, short turn, where few groups have anything, from being ranked whole.  A later
+            // logit that is equal to it comes behind it.
+            const unsigned long long so_far = best[0][p.top - 1];
+            const unsigned above = so_far ? ((unsigned)(so_far >> 32) + 1) << 16 : 0, least = found.bound > above ? found.bound : above;
+            const __half least_x = least ? value_of(least >> 16) : __ushort_as_half((unsigned short)0xFBFF);  // the lowest f16
             if (mine >= __half2float(least_x)) {
                 const __half2 least2 = __half2half2(least_x);
+                unsigned hit = 0;
 #pragma unroll
-                for (int e = 0; e < PIECES * 4; e++) {
-                    const unsigned hit = __hge2_mask(v[e], least2);
-                    if (hit == 0) continue;
-                    const unsigned at = (unsigned)((p0 + tid + (e >> 2) * kTopThreads) * 8 + 2 * (e & 3) - ahead);
-                    const unsigned long long a = key_of(__low2half(v[e]), at), b = key_of(__high2half(v[e]), at + 1);
-                    if ((hit & 0xFFFFu) && a >= least) list[atomicAdd(&n_list, 1)] = a;
-                    if (hit >> 16 && b >= least) list[atomicAdd(&n_list, 1)] = b;
+                for (int e = 0; e < PIECES * 4; e++) hit |= __hge2_mask(v[e], least2) & (0x10001u << e);
+#pragma unroll 1
+                while (hit) {
+                    const int bit = __ffs(hit) - 1;
+                    hit &= hit - 1;
+                    const unsigned key = key_of(value_at(bit & 15, bit >> 4), bit & 15, bit >> 4);
+                    if (key >= least) list[atomicAdd(&found.n, 1)] = key;
                 }
             }
         }
@@ -468,12 +459,34 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
             t += warp_t[w];
         }
         joined(run, {c, s, t});
-        {
+        __syncthreads();
+        // a warp a key: how many are larger
+        const int n = found.n;
+#pragma unroll 1
+        for (int i = warp; i < n; i += kTopWarps) {
+            const unsigned key = list[i];
+            int above = 0;
+#pragma unroll 1
+            for (int j = lane; j - lane < n && above < p.top; j += 32) above += __popc(__ballot_sync(0xffffffffu, j < n && list[j] > key));
+            if (lane == 0 && above < p.top) turn_best[above] = key;
+        }
+        __syncthreads();
+        auto whole = [&](unsigned key) {
+            const unsigned id = (unsigned)(p0 * 8 - ahead) + (0xFFFF - (key & 0xFFFF));
+            return key ? (unsigned long long)(key >> 16) << 32 | (0xFFFFFFFFu - id) : 0;
+        };
+        if (p0 == first) {
+            if (tid < p.top) best[0][tid] = whole(turn_best[tid]);
+        } else {
+            // two sorted lists, a warp each: a key's place is its own and the number of larger ones in the other
+            unsigned long long key = 0;
+            int above = lane;
+            if (warp < 2 && lane < p.top) {
+                key = warp ? whole(turn_best[lane]) : best[0][lane];
+                for (int i = 0; i < p.top; i++) above += (warp ? best[0][i] : whole(turn_best[i])) > key;
+            }
             __syncthreads();
-            const int n = n_list;
-            if (tid < p.top) best[0][tid] = 0;
-            __syncthreads();
-            ranked(list, n, p.top, [&](unsigned long long key, int i, int above) { best[0][above] = key; });
+            if (key > 0 && above < p.top) best[0][above] = key;
         }
     }
     // The first CTA of the row joins what the others found.
@@ -497,25 +510,48 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank > 0) return;
         for (int i = 1; i < p.cluster; i++) joined(run, sums[i]);
-    } else {
-        __syncthreads();
     }
     if (tid == 0) store_row(p, row, target, run);
     const float log2_s = run.c < INFINITY ? log2f(run.s) : 0.f;
-    // the best of all CTAs' best, which lie end to end
-    const int n = p.cluster * p.top;
     const size_t out = (size_t)row * p.top;
+    auto store = [&](int at, unsigned long long key) {
+        p.top_ids[out + at] = (int)(0xFFFFFFFFu - (unsigned)key);  // (of no logit: -1)
+        p.top_logprobs[out + at] = key ? logprob_of(__half2float(value_of((unsigned)(key >> 32))), run, log2_s) : -INFINITY;
+    };
     __syncthreads();
-    for (int i = tid; i < n; i += kTopThreads) list[i] = best[i / p.top][i % p.top];
-    if (tid < p.top) {
-        p.top_ids[out + tid] = -1;
-        p.top_logprobs[out + tid] = -INFINITY;
+    if (p.cluster == 1) {
+        if (tid < p.top) store(tid, best[0][tid]);
+        return;
     }
+    // The CTAs' sorted lists: a key's place is the number of larger ones in each, a thread a list.
+    if (tid < p.top) store(tid, 0);
     __syncthreads();
-    ranked(list, n, p.top, [&](unsigned long long key, int i, int above) {
-        p.top_ids[out + above] = (int)(0xFFFFFFFFu - (unsigned)key);
-        p.top_logprobs[out + above] = logprob_of(__half2float(value_of(key)), run, log2_s);
-    });
+    for (int i = tid; i < p.cluster * p.cluster * kMaxTop; i += kTopThreads) {
+        const int other = i & (p.cluster - 1), item = i / p.cluster, mine = item / kMaxTop, at = item % kMaxTop;
+        const unsigned long long key = at < p.top ? best[mine][at] : 0;
+        int low = other == mine ? at : 0, high = other == mine ? at : p.top;
+        while (low < high) {
+            const int mid = (low + high) / 2;
+            if (best[other][mid] > key) low = mid + 1;
+            else high = mid;
+        }
+        for (int o = 1; o < p.cluster; o *= 2) low += __shfl_xor_sync(0xffffffffu, low, o);
+        if (other == 0 && key > 0 && low < p.top) store(low, key);
+    }
+}
+
+template <int PIECES>
+cudaError_t launch_top(tlc_ctx *ctx, cudaLaunchConfig_t &cfg, const LogprobParams &p) {
+    constexpr size_t smem = list_size<PIECES>() * sizeof(unsigned);
+    static bool configured[64] = {};
+    if (!configured[ctx->device & 63]) {
+        const cudaError_t e = cudaFuncSetAttribute(logprob_top_kernel<PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        configured[ctx->device & 63] = true;
+    }
+    cfg.blockDim = dim3(kTopThreads);
+    cfg.dynamicSmemBytes = smem;
+    return cudaLaunchKernelEx(&cfg, logprob_top_kernel<PIECES>, p);
 }
 
 // How many 16-byte pieces a slice has, at most.
@@ -544,20 +580,6 @@ int ctas_a_row(int sms, int rows, int vocab, bool alternatives) {
         }
     }
     return best;
-}
-
-template <int PIECES>
-cudaError_t launch_top(tlc_ctx *ctx, cudaLaunchConfig_t &cfg, const LogprobParams &p) {
-    constexpr size_t smem = list_size<PIECES>() * sizeof(unsigned long long);
-    static bool configured[64] = {};
-    if (!configured[ctx->device & 63]) {
-        const cudaError_t e = cudaFuncSetAttribute(logprob_top_kernel<PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-        configured[ctx->device & 63] = true;
-    }
-    cfg.blockDim = dim3(kTopThreads);
-    cfg.dynamicSmemBytes = smem;
-    return cudaLaunchKernelEx(&cfg, logprob_top_kernel<PIECES>, p);
 }
 
 }  // namespace
