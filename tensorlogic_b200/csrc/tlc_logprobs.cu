@@ -20,6 +20,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kUnroll = 4;  // 16-byte pieces of a thread in flight, twice
 constexpr float kLow = -60000.f;  // 2^y of the lowest f16 is zero beside any value from here on
 constexpr int kTopThreads = 512, kTopWarps = kTopThreads / 32, kGroups = 64;
+constexpr int kTargetThread = 64;  // (the first threads have the row's first piece and the merging)
 constexpr int kMaxTop = 32, kMaxCluster = 8;
 // what k groups of threads with so many 16-byte pieces each hold
 template <int PIECES> constexpr int list_size() { return kMaxTop * (kTopThreads / kGroups) * PIECES * 8; }
@@ -36,7 +37,7 @@ struct LogprobParams {
     const int *targets;
     float *logprobs, *entropy, *top_logprobs;
     int *top_ids;
-    int rows, vocab, top, cluster;
+    int rows, vocab, top, cluster, cluster_log2;
     tlc_dev_status *status;
 };
 struct Sums {
@@ -53,7 +54,7 @@ __device__ __forceinline__ void moved_to(Sums &a, float c) {
 
 // Log probability of a logit, and what a row without alternatives returns.
 __device__ __forceinline__ float logprob_of(float x, const Sums &run, float log2_s) { return (fmaf(x, kLog2e, run.c) - log2_s) * kLn2; }
-struct Target {  // fetched at the start: two trips to memory, one behind the other
+struct Target {  // fetched behind the first loads: two trips to memory, one behind the other
     int id;
     float x;
 };
@@ -104,12 +105,12 @@ __device__ __forceinline__ void joined(Sums &run, Sums a) {
 struct Row {
     const __half *base, *lo, *hi;
     int ahead, vocab;  // values of the first piece in front of the row
-    long long pieces;
+    int pieces;
     // Its values of a piece; -inf for what is not finite or not the row's.
-    __device__ __forceinline__ uint4 load(long long at, long long end) const {
+    __device__ __forceinline__ uint4 load(int at, int end) const {
         uint4 w = make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
         if (at >= end) return w;
-        const __half *src = base + at * 8;
+        const __half *src = base + (size_t)at * 8;
         if (src >= lo && src + 8 <= hi) {
             w = *reinterpret_cast<const uint4 *>(src);
         } else {
@@ -122,12 +123,12 @@ struct Row {
         return w;
     }
     // A piece without what is not the row's: -inf in its place.
-    __device__ __forceinline__ uint4 own(uint4 w, long long at) const {
+    __device__ __forceinline__ uint4 own(uint4 w, int at) const {
         if (at != 0 && at + 1 != pieces) return w;
         unsigned m[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const long long i = at * 8 + 2 * e - ahead;
+            const long long i = (long long)at * 8 + 2 * e - ahead;
             if (i < 0 || i >= vocab) m[e] = (m[e] & 0xFFFF0000u) | 0xFC00u;
             if (i + 1 < 0 || i + 1 >= vocab) m[e] = (m[e] & 0xFFFFu) | 0xFC000000u;
         }
@@ -153,19 +154,17 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
     if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     tlc_pdl_after_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = blockIdx.x % p.cluster, row = blockIdx.x / p.cluster;
+    const int rank = blockIdx.x & (p.cluster - 1), row = blockIdx.x >> p.cluster_log2;
     const __half *x0 = p.logits + (size_t)row * p.vocab;
     Target target = {-1, 0.f};
-    if (tid == 0 && rank == 0) target = target_of(p, row);
     Row r;
     r.ahead = (int)(((uintptr_t)x0 & 15) >> 1);
     r.vocab = p.vocab;
     r.base = x0 - r.ahead;
     r.lo = p.logits;
     r.hi = p.logits + (size_t)p.rows * p.vocab;
-    r.pieces = ((long long)r.ahead + p.vocab + 7) / 8;
-    const long long share = (r.pieces + p.cluster - 1) / p.cluster, first = rank * share,
-                    end = first + share < r.pieces ? first + share : r.pieces;
+    r.pieces = (int)(((unsigned)r.ahead + p.vocab + 7) / 8);
+    const int share = (r.pieces + p.cluster - 1) >> p.cluster_log2, first = rank * share, end = min(first + share, r.pieces);
 
     // ---- one pass: the thread's largest value and its sums ----
     Sums run = {INFINITY, 0.f, 0.f};
@@ -174,18 +173,19 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
         // 1024 pieces a turn.  Turns within the row need no look at its ends.
         constexpr int kTurn = kUnroll * kThreads;
         uint4 w[kUnroll];
-        auto inside = [&](long long turn) { return turn > 0 && turn + kTurn < r.pieces && turn + kTurn <= end; };
-        auto load = [&](long long turn) {
+        auto inside = [&](int turn) { return turn > 0 && turn + kTurn < r.pieces && turn + kTurn <= end; };
+        auto load = [&](int turn) {
             if (inside(turn)) {
 #pragma unroll
-                for (int i = 0; i < kUnroll; i++) w[i] = *reinterpret_cast<const uint4 *>(r.base + (turn + tid + i * kThreads) * 8);
+                for (int i = 0; i < kUnroll; i++) w[i] = *reinterpret_cast<const uint4 *>(r.base + (size_t)(turn + tid + i * kThreads) * 8);
             } else {
 #pragma unroll
                 for (int i = 0; i < kUnroll; i++) w[i] = r.load(turn + tid + i * kThreads, end);
             }
         };
         load(first);
-        for (long long turn = first; turn < end; turn += kTurn) {
+        if (tid == 0 && rank == 0) target = target_of(p, row);
+        for (int turn = first; turn < end; turn += kTurn) {
             if (!inside(turn)) {
 #pragma unroll
                 for (int i = 0; i < kUnroll; i++) w[i] = r.own(w[i], turn + tid + i * kThreads);
@@ -204,9 +204,10 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
             if (fmaxf(m, most) < kLow) {
 #pragma unroll 1
                 for (int i = 0; i < kUnroll * 8; i++) {
-                    const long long at = turn + tid + (i >> 3) * kThreads, n = at * 8 + (i & 7) - r.ahead;
+                    const int at = turn + tid + (i >> 3) * kThreads;
+                    const long long n = (long long)at * 8 + (i & 7) - r.ahead;
                     if (at >= end || n < 0 || n >= r.vocab) continue;
-                    const float x = __half2float(r.base[at * 8 + (i & 7)]);
+                    const float x = __half2float(r.base[(size_t)at * 8 + (i & 7)]);
                     if (!isfinite(x)) continue;
                     if (x > most) {
                         most = x;
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     constexpr int kTurn = kTopThreads * PIECES;  // pieces
     extern __shared__ __align__(16) unsigned list[];  // [list_size<PIECES>()]
     __shared__ __align__(16) unsigned group_best[kGroups];
-    __shared__ __align__(16) unsigned long long best[kMaxCluster][kMaxTop];  // of this CTA's turns; in the first CTA, of all
+    __shared__ __align__(16) unsigned long long best[kMaxCluster][kMaxTop + 1];  // of this CTA's turns; in the first CTA, of all (its lists in different banks)
     __shared__ __align__(16) unsigned turn_best[kMaxTop];
     __shared__ __align__(16) Sums sums[kMaxCluster];
     __shared__ __align__(16) float warp_max[kTopWarps], warp_s[kTopWarps], warp_t[kTopWarps];
@@ -311,46 +312,45 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     tlc_pdl_after_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = blockIdx.x % p.cluster, row = blockIdx.x / p.cluster;
+    const int rank = blockIdx.x & (p.cluster - 1), row = blockIdx.x >> p.cluster_log2;
     const __half *x0 = p.logits + (size_t)row * p.vocab;
     Target target = {-1, 0.f};
-    if (tid == 0 && rank == 0) target = target_of(p, row);
     // The row in 16-byte pieces of memory: the first and the last may reach into other rows, and past the array.
     const int ahead = (int)(((uintptr_t)x0 & 15) >> 1);  // values of the first piece in front of the row
     const __half *base = x0 - ahead;
-    const long long pieces = ((long long)ahead + p.vocab + 7) / 8, share = (pieces + p.cluster - 1) / p.cluster;
-    const long long first = rank * share, end = first + share < pieces ? first + share : pieces;
+    const int pieces = (int)(((unsigned)ahead + p.vocab + 7) / 8), share = (pieces + p.cluster - 1) >> p.cluster_log2;
+    const int first = rank * share, end = min(first + share, pieces);
+    const int whole_first = ahead > 0, whole_end = (int)(((unsigned)ahead + p.vocab) / 8);  // pieces that are all the row's
 
     if (tid < p.top) best[0][tid] = 0;
     if (tid < kGroups) group_best[tid] = 0;
     Sums run = {INFINITY, 0.f, 0.f};
-    for (long long p0 = first; p0 < end; p0 += kTurn) {
+    for (int p0 = first; p0 < end; p0 += kTurn) {
         __half2 v[PIECES * 4];
         {
             uint4 w[PIECES];
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
-                const long long at = p0 + tid + i * kTopThreads;
+                const int at = p0 + tid + i * kTopThreads;
                 w[i] = make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);  // -inf
-                if (at > 0 && at + 1 < pieces && at < end) w[i] = *reinterpret_cast<const uint4 *>(base + at * 8);
+                if (at >= whole_first && at < whole_end && at < end) w[i] = *reinterpret_cast<const uint4 *>(base + (size_t)at * 8);
             }
-            // the row's first and last piece, value by value
+            // a first and a last piece of which the row has a part, value by value
 #pragma unroll 1
-            for (int side = 0; side < 2; side++) {
-                const long long at = side ? pieces - 1 : 0, off = at - p0 - tid;
+            for (int at = whole_first ? 0 : whole_end; at < pieces; at = at < whole_end ? whole_end : pieces) {
+                const int off = at - p0 - tid;
                 if (at >= end || off < 0 || off >= kTurn || (off & (kTopThreads - 1))) continue;
-                unsigned long long low = 0, high = 0;
-#pragma unroll 1
+                unsigned x[8];
+#pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const long long n = at * 8 + e - ahead;
-                    const unsigned long long x = n >= 0 && n < p.vocab ? __half_as_ushort(x0[n]) : 0xFC00;
-                    low = low >> 16 | high << 48;
-                    high = high >> 16 | x << 48;
+                    const long long n = (long long)at * 8 + e - ahead;
+                    x[e] = n >= 0 && n < p.vocab ? __half_as_ushort(x0[n]) : 0xFC00;
                 }
 #pragma unroll
                 for (int i = 0; i < PIECES; i++)
-                    if (off == i * kTopThreads) w[i] = make_uint4((unsigned)low, (unsigned)(low >> 32), (unsigned)high, (unsigned)(high >> 32));
+                    if (off == i * kTopThreads) w[i] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
             }
+            if (p0 == 0 && tid == kTargetThread) target = target_of(p, row);
 #pragma unroll
             for (int i = 0; i < PIECES; i++) clean(w[i], __float2half2_rn(-INFINITY), *reinterpret_cast<__half2(*)[4]>(&v[4 * i]));
         }
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
         }
         __syncthreads();
         auto whole = [&](unsigned key) {
-            const unsigned id = (unsigned)(p0 * 8 - ahead) + (0xFFFF - (key & 0xFFFF));
+            const unsigned id = ((unsigned)p0 * 8 - ahead) + (0xFFFF - (key & 0xFFFF));
             return key ? (unsigned long long)(key >> 16) << 32 | (0xFFFFFFFFu - id) : 0;
         };
         if (p0 == first) {
@@ -489,6 +489,11 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
             if (key > 0 && above < p.top) best[0][above] = key;
         }
     }
+    const size_t out = (size_t)row * p.top;
+    if (rank == 0 && tid < p.top) {  // where there are fewer logits
+        p.top_ids[out + tid] = -1;
+        p.top_logprobs[out + tid] = -INFINITY;
+    }
     // The first CTA of the row joins what the others found.
     if (p.cluster > 1) {
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the row runs
@@ -498,7 +503,9 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
             asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)));
             return a;
         };
-        if (rank > 0) {
+        if (rank == 0) {
+            if (tid == 0) sums[0] = run;
+        } else {
             if (tid < p.top)
                 asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&best[rank][tid])), "l"(best[0][tid]) : "memory");
             if (tid < 3)
@@ -509,35 +516,39 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank > 0) return;
-        for (int i = 1; i < p.cluster; i++) joined(run, sums[i]);
+        run = lane < p.cluster ? sums[lane] : Sums{INFINITY, 0.f, 0.f};
+        warp_sums(run);
     }
-    if (tid == 0) store_row(p, row, target, run);
     const float log2_s = run.c < INFINITY ? log2f(run.s) : 0.f;
-    const size_t out = (size_t)row * p.top;
     auto store = [&](int at, unsigned long long key) {
-        p.top_ids[out + at] = (int)(0xFFFFFFFFu - (unsigned)key);  // (of no logit: -1)
-        p.top_logprobs[out + at] = key ? logprob_of(__half2float(value_of((unsigned)(key >> 32))), run, log2_s) : -INFINITY;
+        p.top_ids[out + at] = (int)(0xFFFFFFFFu - (unsigned)key);
+        p.top_logprobs[out + at] = logprob_of(__half2float(value_of((unsigned)(key >> 32))), run, log2_s);
     };
     __syncthreads();
     if (p.cluster == 1) {
-        if (tid < p.top) store(tid, best[0][tid]);
-        return;
-    }
-    // The CTAs' sorted lists: a key's place is the number of larger ones in each, a thread a list.
-    if (tid < p.top) store(tid, 0);
-    __syncthreads();
-    for (int i = tid; i < p.cluster * p.cluster * kMaxTop; i += kTopThreads) {
-        const int other = i & (p.cluster - 1), item = i / p.cluster, mine = item / kMaxTop, at = item % kMaxTop;
-        const unsigned long long key = at < p.top ? best[mine][at] : 0;
-        int low = other == mine ? at : 0, high = other == mine ? at : p.top;
-        while (low < high) {
-            const int mid = (low + high) / 2;
-            if (best[other][mid] > key) low = mid + 1;
-            else high = mid;
+        if (tid < p.top && best[0][tid] > 0) store(tid, best[0][tid]);
+    } else {
+        // The CTAs' sorted lists: a key's place is the number of larger ones in each, a thread a list, up to four at once.
+        const int other = tid & (p.cluster - 1), step = kTopThreads >> p.cluster_log2, n = p.cluster * kMaxTop;
+        unsigned long long key[4];
+        int place[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int item = (tid >> p.cluster_log2) + i * step, at = item % kMaxTop;
+            key[i] = item < n && at < p.top ? best[item / kMaxTop][at] : 0;
         }
-        for (int o = 1; o < p.cluster; o *= 2) low += __shfl_xor_sync(0xffffffffu, low, o);
-        if (other == 0 && key > 0 && low < p.top) store(low, key);
+#pragma unroll
+        for (int jump = kMaxTop; jump > 0; jump /= 2)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (place[i] + jump <= p.top && best[other][place[i] + jump - 1] > key[i]) place[i] += jump;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            for (int o = 1; o < p.cluster; o *= 2) place[i] += __shfl_xor_sync(0xffffffffu, place[i], o);
+            if (other == 0 && key[i] > 0 && place[i] < p.top) store(place[i], key[i]);
+        }
     }
+    if (tid == kTargetThread) store_row(p, row, target, run);
 }
 
 template <int PIECES>
@@ -564,12 +575,12 @@ constexpr long long slice_pieces(int vocab, int ctas) { return ((long long)vocab
 // share SMs and cost 0.85 of that.  37 x 32000 with alternatives takes 8.6 us with 2 CTAs a row, 9.8 with 4 and 14.7
 // with 8; 37 x 100003 21.7, 18.1 and 18.5; 148 x 100003 32.4, 43.9 and 51.2.
 int ctas_a_row(int sms, int rows, int vocab, bool alternatives) {
-    constexpr double kJoin[2][4] = {{0, 1.1, 1.3, 2.1}, {0, 0.6, 0.7, 1.6}};
+    constexpr double kJoin[2][4] = {{0, 1.1, 1.3, 2.1}, {0, 1.2, 1.4, 1.6}};
     int best = 1;
     double least = 1e30;
     for (int c = 1, i = 0; c <= kMaxCluster; c *= 2, i++) {
         const long long n = slice_pieces(vocab, c), held = n <= kTopThreads ? 1 : n <= 2 * kTopThreads ? 2 : 4;
-        const double work = alternatives ? (double)((n + held * kTopThreads - 1) / (held * kTopThreads)) * (2.6 + 0.45 * held) : n * 8 / 15000.0;
+        const double work = alternatives ? (double)((n + held * kTopThreads - 1) / (held * kTopThreads)) * (1.5 + 0.49 * held) : n * 8 / 15000.0;
         int at_once = (c <= 2 ? sms : sms * 4 / 5) / c;
         if (at_once < 1) at_once = 1;
         const int layers = (rows - 1) / at_once + 1;
@@ -609,6 +620,7 @@ extern "C" int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int3
     p.status = ctx->dev_status;
     const int c = ctas_a_row(ctx->sm_count, rows, vocab, top_k > 0);
     p.cluster = c;
+    while (1 << p.cluster_log2 < c) p.cluster_log2++;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * c));
     cfg.blockDim = dim3(kThreads);
