@@ -294,6 +294,20 @@ __device__ __forceinline__ __half value_of(unsigned v) {
     return __ushort_as_half((v & 0x8000) ? (unsigned short)(v & 0x7FFF) : (unsigned short)~v);
 }
 
+// take(key, how many are larger) for those of n keys that fewer than `top` are larger than, a warp a key.
+template <typename K, typename F>
+__device__ __forceinline__ void ranked(const K *keys, int n, int top, F &&take) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int i = threadIdx.x >> 5; i < n; i += kTopWarps) {
+        const K key = keys[i];
+        int above = 0;
+#pragma unroll 1
+        for (int j = lane; j - lane < n && above < top; j += 32) above += __popc(__ballot_sync(0xffffffffu, j < n && keys[j] > key));
+        if (lane == 0 && above < top) take(key, above);
+    }
+}
+
 // With alternatives.
 template <int PIECES>
 __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const LogprobParams p) {
@@ -460,16 +474,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
         }
         joined(run, {c, s, t});
         __syncthreads();
-        // a warp a key: how many are larger
-        const int n = found.n;
-#pragma unroll 1
-        for (int i = warp; i < n; i += kTopWarps) {
-            const unsigned key = list[i];
-            int above = 0;
-#pragma unroll 1
-            for (int j = lane; j - lane < n && above < p.top; j += 32) above += __popc(__ballot_sync(0xffffffffu, j < n && list[j] > key));
-            if (lane == 0 && above < p.top) turn_best[above] = key;
-        }
+        ranked(list, found.n, p.top, [&](unsigned key, int above) { turn_best[above] = key; });
         __syncthreads();
         auto whole = [&](unsigned key) {
             const unsigned id = ((unsigned)p0 * 8 - ahead) + (0xFFFF - (key & 0xFFFF));
@@ -504,7 +509,10 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
             return a;
         };
         if (rank == 0) {
-            if (tid == 0) sums[0] = run;
+            if (tid == 0) {
+                sums[0] = run;
+                found.n = 0;
+            }
         } else {
             if (tid < p.top)
                 asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&best[rank][tid])), "l"(best[0][tid]) : "memory");
@@ -528,25 +536,14 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     if (p.cluster == 1) {
         if (tid < p.top && best[0][tid] > 0) store(tid, best[0][tid]);
     } else {
-        // The CTAs' sorted lists: a key's place is the number of larger ones in each, a thread a list, up to four at once.
-        const int other = tid & (p.cluster - 1), step = kTopThreads >> p.cluster_log2, n = p.cluster * kMaxTop;
-        unsigned long long key[4];
-        int place[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int item = (tid >> p.cluster_log2) + i * step, at = item % kMaxTop;
-            key[i] = item < n && at < p.top ? best[item / kMaxTop][at] : 0;
-        }
-#pragma unroll
-        for (int jump = kMaxTop; jump > 0; jump /= 2)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (place[i] + jump <= p.top && best[other][place[i] + jump - 1] > key[i]) place[i] += jump;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            for (int o = 1; o < p.cluster; o *= 2) place[i] += __shfl_xor_sync(0xffffffffu, place[i], o);
-            if (other == 0 && key[i] > 0 && place[i] < p.top) store(place[i], key[i]);
-        }
+        // The CTAs' sorted lists: k keys reach the least of their (k / CTAs)-th ones, and no key below it counts.
+        unsigned long long *keys = reinterpret_cast<unsigned long long *>(list), least = ~0ull;
+        const int nth = (p.top + p.cluster - 1) >> p.cluster_log2, at = tid % kMaxTop;
+        for (int i = 0; i < p.cluster; i++) least = min(least, best[i][nth - 1]);
+        const unsigned long long key = tid < p.cluster * kMaxTop && at < p.top ? best[tid / kMaxTop][at] : 0;
+        if (key > 0 && key >= least) keys[atomicAdd(&found.n, 1)] = key;
+        __syncthreads();
+        ranked(keys, found.n, p.top, [&](unsigned long long key, int above) { store(above, key); });
     }
     if (tid == kTargetThread) store_row(p, row, target, run);
 }
