@@ -147,7 +147,8 @@ __device__ __forceinline__ void clean(uint4 w, __half2 none, __half2 (&v)[4]) {
     }
 }
 
-// Without alternatives.
+// Without alternatives.  512 x 32000 takes 9.3 us (3.5 TB/s out of the L2 and HBM, 54 % of the copy's rate): 33 MB of
+// loads with 64 KB in flight an SM, and about 7 instructions a logit.
 __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParams p) {
     __shared__ Sums sums[kMaxCluster];
     __shared__ float warp_c[kWarps], warp_s[kWarps], warp_t[kWarps];
@@ -308,7 +309,11 @@ __device__ __forceinline__ void ranked(const K *keys, int n, int top, F &&take) 
     }
 }
 
-// With alternatives.
+// With alternatives.  Bound by latencies: of a turn's 8000 cycles (1 x 100003 split eight ways) 1500 pass until the
+// logits are there, 1200 in the exponentials (16384, at 16 a cycle of the SM), the rest between barriers -- bound,
+// candidates, ranks -- and 2000 more in joining the cluster, 1700 in ranking what its CTAs found.  512 threads halve
+// the steps of each against 256 and leave room for a second CTA on the SM.  1 x 32000 with 5 alternatives takes 4.7 us, of
+// which a call's launch is 3.6; 37 x 100003 with 20 12.2.
 template <int PIECES>
 __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const LogprobParams p) {
     constexpr int kTurn = kTopThreads * PIECES;  // pieces
@@ -566,11 +571,11 @@ cudaError_t launch_top(tlc_ctx *ctx, cudaLaunchConfig_t &cfg, const LogprobParam
 constexpr long long slice_pieces(int vocab, int ctas) { return ((long long)vocab + 14) / 8 / ctas + 1; }
 
 // CTAs a row, by cost in microseconds as fitted to calls of 1 to 400 rows of 16000 to 151936 logits with 1, 2, 4 and 8
-// CTAs a row.  A row costs the joining of its CTAs and a CTA's work: a turn of 2048 pieces with alternatives (4.4, a
-// slice held in 1 or 2 pieces a thread 3.05 or 3.5), 15000 logits a microsecond without.  As many clusters as find an SM
-// for each CTA run at once (4 or 8 CTAs must lie in one part of the chip: a fifth of the SMs stays empty); further ones
-// share SMs and cost 0.85 of that.  37 x 32000 with alternatives takes 8.6 us with 2 CTAs a row, 9.8 with 4 and 14.7
-// with 8; 37 x 100003 21.7, 18.1 and 18.5; 148 x 100003 32.4, 43.9 and 51.2.
+// CTAs a row.  A row costs the joining of its CTAs and a CTA's work: a turn of 2048 pieces with alternatives (3.45, with
+// 512 or 1024 pieces 2 or 2.5), 15000 logits a microsecond without.  As many clusters as find an SM for each CTA run at
+// once (4 or 8 CTAs must lie in one part of the chip: a fifth of the SMs stays empty); further ones share SMs and cost
+// 0.8 of that.  With 20 alternatives 36 x 32000 takes 8.9, 6.5, 7.2 and 9.7 us with 1, 2, 4 and 8 CTAs a row, 36 x 100003
+// 27.0, 17.5, 13.8 and 12.2, 148 x 100003 30.3, 25.1, 32.1 and 32.6.
 int ctas_a_row(int sms, int rows, int vocab, bool alternatives) {
     constexpr double kJoin[2][4] = {{0, 1.1, 1.3, 2.1}, {0, 1.2, 1.4, 1.6}};
     int best = 1;
@@ -581,7 +586,7 @@ int ctas_a_row(int sms, int rows, int vocab, bool alternatives) {
         int at_once = (c <= 2 ? sms : sms * 4 / 5) / c;
         if (at_once < 1) at_once = 1;
         const int layers = (rows - 1) / at_once + 1;
-        const double cost = kJoin[alternatives][i] + work * (layers == 1 ? 1 : 0.85 * layers);
+        const double cost = kJoin[alternatives][i] + work * (layers == 1 ? 1 : 0.8 * layers);
         if (cost < least) {
             least = cost;
             best = c;
