@@ -112,11 +112,30 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
     const uint8_t *codes = p.c.codes + head * p.c.n_blocks * (2 * STAGE);
     const float2 *scales = reinterpret_cast<const float2 *>(p.c.scales) + head * p.c.n_blocks;
 
-    // The ring: K and V of a block in turn.
+    // The ring: K and V of a block in turn.  Rows of 128 values: at the end the open block's, where this warp's turn comes
+    // to it, f16, two stages of 32 keys each, and only the 16-key groups that anyone sees (32 sequences of about 600 keys,
+    // 32 heads: 35.8 us with all of them read straight from memory behind the ring, 32.9 so).  Rows of 64: all of the open
+    // block's loads at once, behind the ring (a token behind 512, 32 heads: 5.6 us so, 5.9 through the ring).
+    constexpr bool kOpenInRing = D == 128;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)(warp * ST * STAGE + lane * 16);
     const int n_sealed = min(units, sealed), steps = u0 < n_sealed ? 2 * ((n_sealed - u0 + stride - 1) / stride) : 0;
+    const bool has_open = kOpenInRing && units > sealed && u0 + (steps >> 1) * stride == sealed;
+    const int groups = has_open ? (seen - sealed * kKv8Block + 15) / 16 : 0;
+    const uint8_t *open = reinterpret_cast<const uint8_t *>(p.c.open + head * (2 * STAGE));
     auto fetch = [&](int n) {
-        if (n < steps) {
+        if constexpr (kOpenInRing) {
+            const int part = n - steps, have = part < 0 ? 2 : part < 4 ? groups - 2 * (part & 1) : 0;  // halves of a stage
+            const uint8_t *src = (part < 0 ? codes + ((size_t)(u0 + (n >> 1) * stride) * 2 + (n & 1)) * STAGE : open + part * STAGE) + lane * 16;
+            const uint32_t dst = ring + (uint32_t)(n % ST * STAGE);
+            if (have > 0) {
+#pragma unroll
+                for (int i = 0; i < LOADS / 2; i++) copy16(dst + i * 512, src + i * 512);
+            }
+            if (have > 1) {
+#pragma unroll
+                for (int i = LOADS / 2; i < LOADS; i++) copy16(dst + i * 512, src + i * 512);
+            }
+        } else if (n < steps) {
             const uint8_t *src = codes + ((size_t)(u0 + (n >> 1) * stride) * 2 + (n & 1)) * STAGE + lane * 16;
             const uint32_t dst = ring + (uint32_t)(n % ST * STAGE);
 #pragma unroll
@@ -312,8 +331,55 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
         }
         step++;
     }
-    // The open block, where this warp's turn has come to it: f16 rows straight from memory.
-    if (units > sealed && sealed % stride == u0) {
+    // The open block
+    if (kOpenInRing && has_open) {
+        float s[4][NT][4], psum[NT][2], corr[NT][2];
+        const float none[NT][2] = {};
+        uint32_t pf[4][NT][2];
+#pragma unroll
+        for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) s[kg][nt][0] = s[kg][nt][1] = s[kg][nt][2] = s[kg][nt][3] = 0.f;
+        // (What a group that was not copied leaves of its scores is masked; of V it counts as zeros.)
+        auto at = [&](int half) { return ring + (uint32_t)((step + half) % ST * STAGE); };
+        fetch(step + ST - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+#pragma unroll
+        for (int k16 = 0; k16 < D / 16; k16++) {
+            uint4 w[4];
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++) w[kg] = lds128(at(kg >> 1) + (uint32_t)(((kg & 1) * (D / 16) + k16) * 512));
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma(s[kg][nt], w[kg].x, w[kg].z, w[kg].y, w[kg].w, qf[nt][k16][0], qf[nt][k16][1]);
+        }
+        step += 2;
+        fetch(step + ST - 2);
+        fetch(step + ST - 1);
+        softmax(sealed, s, p.scale * kLog2e, pf, psum, corr);
+        reduce(psum, corr);
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+#pragma unroll
+        for (int dt = 0; dt < D / 16; dt++) {
+            float acc[NT][4];
+            uint4 w[4];
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++) {
+                w[kg] = lds128(at(kg >> 1) + (uint32_t)(((kg & 1) * (D / 16) + dt) * 512));
+                if (kg >= groups) w[kg] = make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma(acc[nt], w[kg].x, w[kg].z, w[kg].y, w[kg].w, pf[kg][nt][0], pf[kg][nt][1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) join(dt, nt, acc[nt], 1.f, none, corr);
+        }
+    }
+    if (!kOpenInRing && units > sealed && sealed % stride == u0) {
         const uint4 *kt = reinterpret_cast<const uint4 *>(p.c.open + head * (2 * STAGE)) + lane, *vt = kt + STAGE / 8;
         float s[4][NT][4], psum[NT][2], corr[NT][2];
         const float none[NT][2] = {};
