@@ -11,6 +11,9 @@ builtins of the TensorLogic project:
     embedding(table, ids)     src/interpreter/builtin_nn.rs:627-909
     mul / add                 src/ops/elementwise.rs:232-330, :48-140
 
+Beside them, without a counterpart there: ``KVCache8`` (a KV cache of 8-bit codes with the attention over it) and
+``token_logprobs`` (how likely a model found given tokens, with alternatives).
+
 Tensors are f16 device buffers handed out by the context's size-class pool;
 weights are ``QTensor`` objects that keep their GGUF blocks in HBM.  Everything
 runs through the C ABI of include/tlcuda.h; nothing here computes on the host.

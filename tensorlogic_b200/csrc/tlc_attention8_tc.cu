@@ -12,6 +12,10 @@
 //
 // Warps:  0  Q, K and V by TMA      1  tensor memory and MMA issue      2-5  softmax, rescale, output
 //
+// Bound by the tiles' way out of the L2: 2048 queries, 32 heads of 128 move 285 MB there in 41 us (7 TB/s; tensor pipe
+// 45 %, as a product of 64 keys takes as long as one of 128), behind 11 us for the image: 55 us a call.  One CTA with twice
+// the rows moves half of it and took 55 to 61 us for the attention alone, its softmax in turn with its own products.
+//
 // All waits are bounded; one that runs out sets the status word and lets the CTA drain, free its tensor memory and
 // return.
 #include <cuda.h>
