@@ -455,7 +455,9 @@ TLC_API int32_t tlc_kvcache8_rows(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
  * negative position marks an idle slot, whose output rows are zeros.  A query at a position whose key the cache
  * does not hold (or at or past max_keys) sees the keys there are, and the next tlc_synchronize reports
  * TLC_ERR_INDEX.  Allocates nothing, except on the first prompt long enough for the tensor-memory kernel (an
- * f16 image of one sequence and layer): make that call before a stream capture. */
+ * f16 image of one sequence and layer); in a stream capture, and where there is no room for it, such a prompt
+ * runs on the other kernel, several times slower: make the first one before a capture.  Calls over one cache
+ * share its workspace and run one after the other, replays of captured ones included. */
 TLC_API int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t layer, const void *q_dev,
                                void *out_dev, int32_t batch, int32_t n_queries, int32_t n_heads,
                                int32_t sequence, int32_t q_pos0, const int32_t *positions_dev,

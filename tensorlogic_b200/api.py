@@ -404,9 +404,10 @@ def token_logprobs(logits: Tensor, tokens=None, top_k: int = 0):
     The alternatives are the ``top_k`` (0 .. 32) largest logits, equal ones in the order of their ids.  A token of -1
     has log probability 0 (padding).  Without ``tokens`` the first result is None.  Logits that are not finite carry
     no probability, as in ``softmax``."""
-    vocab = logits.shape[-1]
-    rows, dev = logits.size // vocab, logits.dev
-    ids_t = None
+    vocab, dev = logits.shape[-1], logits.dev
+    if vocab < 1:
+        raise TensorError(_lib.ERR_INVALID_DIMENSION, f"token_logprobs: bad shape {list(logits.shape)}")
+    rows, ids_t = logits.size // vocab, None
     if tokens is not None:
         ids = np.ascontiguousarray(np.atleast_1d(tokens), dtype=np.int32).reshape(-1)
         if ids.size != rows:
@@ -612,6 +613,8 @@ class KVCache8:
         """get_k / get_v: host copies [len, n_kv_heads, head_dim] of the values the cache stands for."""
         self._check(layer, batch_index, 1)
         n = int(self.lengths[layer, batch_index]) if length is None else length
+        if not 0 <= n <= self.max_seq:
+            raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {n}, size {self.max_seq}")
         out = [self.dev.empty((n, self.n_kv_heads, self.head_dim)) for _ in range(2)]
         check(self.dev.lib.tlc_kvcache8_rows(self.dev.handle, self.handle, layer, batch_index, 1, 0, n, out[0].ptr,
                                              out[1].ptr))

@@ -14,7 +14,7 @@
 //
 // Bound by the tiles' way out of the L2: 2048 queries, 32 heads of 128 move 285 MB there in 41 us (7 TB/s; tensor pipe
 // 45 %, as a product of 64 keys takes as long as one of 128), behind 11 us for the image: 55 us a call.  One CTA with twice
-// the rows moves half of it and took 55 to 61 us for the attention alone, its softmax in turn with its own products.
+// the rows moves half of it and took 55 to 61 us a call, its softmax in turn with its own products.
 //
 // All waits are bounded; one that runs out sets the status word and lets the CTA drain, free its tensor memory and
 // return.
@@ -354,20 +354,24 @@ int32_t launch(tlc_ctx *ctx, const Params &p, const CUtensorMap &q, const CUtens
 
 }  // namespace
 
+bool kv8_image(tlc_ctx *ctx, tlc_kvcache8 *cache) {
+    if (cache->wide) return true;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone) {
+        const size_t rows = (size_t)cache->n_kv_heads * cache->n_blocks * kKv8Block;
+        cudaError_t e = cudaSuccess;
+        if (!cache->factors) e = cudaMalloc(&cache->factors, (size_t)cache->n_kv_heads * cache->n_blocks * sizeof(float4));
+        if (e == cudaSuccess) e = cudaMalloc(&cache->wide, 2 * rows * cache->head_dim * sizeof(__half));
+        if (e == cudaSuccess) return true;
+        cache->wide = nullptr;
+    }
+    cudaGetLastError();
+    return false;
+}
+
 int32_t kv8_attention_tc(tlc_ctx *ctx, tlc_kvcache8 *cache, int layer, int sequence, const __half *q, __half *out, int I, int H,
                          int pos0, float scale) {
     const uint64_t D = cache->head_dim, Hkv = cache->n_kv_heads, rows = (uint64_t)cache->n_blocks * kKv8Block;
-    if (!cache->wide) {
-        cudaError_t e = cudaMalloc(&cache->wide, 2 * Hkv * rows * D * sizeof(__half));
-        if (e == cudaSuccess && !cache->factors) e = cudaMalloc(&cache->factors, Hkv * cache->n_blocks * sizeof(float4));
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            cudaFree(cache->wide);
-            cache->wide = nullptr;
-            return tlc_fail(TLC_ERR_ALLOCATION, "attention8: allocation of %zu bytes failed: %s", (size_t)(2 * Hkv * rows * D * sizeof(__half)),
-                            cudaGetErrorString(e));
-        }
-    }
     Params p{};
     p.out = out;
     p.factors = cache->factors;

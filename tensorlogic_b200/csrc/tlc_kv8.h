@@ -60,6 +60,8 @@ int32_t kv8_check(tlc_ctx *ctx, const tlc_kvcache8 *cache, const char *what, int
 
 // Fills wide and factors with the first `blocks` blocks of a sequence.
 int32_t kv8_widen(tlc_ctx *ctx, tlc_kvcache8 *cache, int layer, int sequence, int blocks);
+// Makes room for them, where there is none yet: not while the stream is being captured, and not if there is no memory.
+bool kv8_image(tlc_ctx *ctx, tlc_kvcache8 *cache);
 // Attention of a prompt over that image on the 5th-generation tensor cores (tlc_attention8_tc.cu).
 int32_t kv8_attention_tc(tlc_ctx *ctx, tlc_kvcache8 *cache, int layer, int sequence, const __half *q, __half *out, int I, int H,
                          int pos0, float scale);

@@ -435,3 +435,49 @@ def test_refusals(dev):
     finally:
         other.close()
     dev.synchronize()
+
+
+@pytest.mark.parametrize("prepared", [False, True])
+def test_captured_prompt(dev, prepared):
+    """A long prompt in a graph: with what its fast kernel keeps made before, and without, where nothing may be made."""
+    import torch
+    from tensorlogic_b200 import _lib
+    from tensorlogic_b200.api import KVCache8
+    H, Hkv, D, I = 8, 2, 128, 900
+    k, v = rows(2, I, Hkv, D)
+    q = queries(2, I, H, D)
+    cache = KVCache8(dev, 1, Hkv, D, max_seq=1000, max_batch=2)
+    cache.append(0, dev.tensor(k), dev.tensor(v), sequence=1)
+    first = cache.attention(0, dev.tensor(q), H, sequence=1).numpy() if prepared else None
+    tq, out = torch.tensor(q, device="cuda"), torch.zeros(I, H, D, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.ExternalStream(dev.stream)):
+        _lib.check(dev.lib.tlc_attention8(dev.handle, cache.handle, 0, tq.data_ptr(), out.data_ptr(), 1, I, H, 1, 0, None, 0, D ** -0.5))
+    g.replay()
+    torch.cuda.synchronize()
+    got = out.cpu().numpy()
+    check_attention(got, q, exact_values(k), exact_values(v), 0)
+    assert not prepared or same(got, first)
+    dev.synchronize()
+
+
+def test_far_into_memory(dev):
+    """The last sequence of the last layer of a cache of more than 2^32 bytes."""
+    from tensorlogic_b200.api import KVCache8
+    H, Hkv, D, B, T = 16, 8, 128, 40, 777
+    cache = KVCache8(dev, 2, Hkv, D, max_seq=32768, max_batch=B)
+    k, v = rows(3, T, Hkv, D)
+    q = queries(3, T, H, D)
+    cache.append(1, dev.tensor(k[:-1]), dev.tensor(v[:-1]), sequence=B - 1)
+    pos = np.array([-1, T - 1])
+    cache.append(1, dev.tensor(np.stack([k[-1]] * 2)), dev.tensor(np.stack([v[-1]] * 2)), positions=pos, sequence=B - 2)
+    got = cache.layer_arrays(1, B - 1)
+    assert same(got[0], held_values(k)) and same(got[1], held_values(v))
+    assert not np.any(cache.layer_arrays(1, B - 2, 5)[0])
+    prompt = cache.attention(1, dev.tensor(q), H, sequence=B - 1).numpy()
+    token = cache.attention(1, dev.tensor(q[-2:]), H, batch=2, positions=pos, sequence=B - 2).numpy()
+    check_attention(prompt, q, exact_values(k), exact_values(v), 0)
+    check_attention(token[1:], q[-1:], exact_values(k), exact_values(v), T - 1)
+    assert not token[0].any()
+    dev.synchronize()

@@ -182,3 +182,27 @@ def test_short_last_slice(dev, vocab):
     for top in (1, 32):
         check(dev, x, rng.integers(0, vocab, 4), top)
     dev.synchronize()
+
+
+@pytest.mark.parametrize("top", [0, 5])
+def test_far_into_memory(dev, top):
+    """The last rows of more than 2^31 logits."""
+    import torch
+    from tensorlogic_b200 import _lib
+    rows, vocab, last = 68000, 32000, 3
+    x = torch.zeros(rows, vocab, dtype=torch.float16, device="cuda")
+    x[-last:] = torch.randn(last, vocab, device="cuda").half() * 3
+    t = torch.arange(rows, dtype=torch.int32, device="cuda") % vocab
+    lp, h, best = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty(rows, 5, device="cuda")
+    ids = torch.empty(rows, 5, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    _lib.check(dev.lib.tlc_token_logprobs(dev.handle, x.data_ptr(), rows, vocab, t.data_ptr(), top, lp.data_ptr(), h.data_ptr(),
+                                          ids.data_ptr() if top else None, best.data_ptr() if top else None))
+    dev.synchronize()
+    host = [a[-last:].cpu().numpy() for a in (x, t, lp, h, ids, best)]
+    for i, (p, e, at, b, tol) in enumerate(oracle(host[0], host[1], top)):
+        assert abs(host[2][i] - p) <= tol[0] + 2.0 ** -22 * abs(p) and abs(host[3][i] - e) <= tol[1]
+        if top:
+            assert list(host[4][i]) == at and all(abs(g - w) <= tol[0] + 2.0 ** -22 * abs(w) for g, w in zip(host[5][i], b))
+    even = np.log(vocab)
+    assert abs(float(lp[0]) + even) <= 2.0 ** -18 + 2.0 ** -22 * even and (lp[:-last] == lp[0]).all() and (h[:-last] == h[0]).all()

@@ -85,3 +85,16 @@ def test_logprob_refusals(fake):
         with pytest.raises(_lib.TensorError):
             token_logprobs(x, tokens, top)
     assert not any(name == "tlc_token_logprobs" for name, _ in fake.lib.calls)
+
+
+def test_shapes_of_nothing(fake):
+    """No rows is no error; no vocabulary, or a length that no sequence can have, is one."""
+    lp, entropy, ids, best = token_logprobs(_tensor(fake, (0, 10)), [], 3)
+    assert lp.shape == entropy.shape == (0,) and ids.shape == best.shape == (0, 3)
+    with pytest.raises(_lib.TensorError):
+        token_logprobs(_tensor(fake, (2, 0)), [0, 0])
+    cache = KVCache8(fake, 1, 2, 64, max_seq=100)
+    for n in (-1, 101):
+        with pytest.raises(_lib.TensorError) as e:
+            cache.layer_arrays(0, 0, n)
+        assert e.value.code == _lib.ERR_INDEX
