@@ -586,7 +586,7 @@ class KVCache8:
         if k.size % row or k.size != v.size:
             raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"KV rows must have {row} elements")
         m = k.size // row
-        self._check(layer, sequence, 1 if positions is None else m)
+        self._check(layer, sequence, 1 if positions is None else m, k, v)
         held = self.lengths[layer, sequence:]
         pos_t = None
         if positions is None:
@@ -627,7 +627,7 @@ class KVCache8:
         D = self.head_dim
         if n_heads < 1 or batch < 1 or q.size % (n_heads * D * batch):
             raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"attention: q has {q.size} elements")
-        self._check(layer, sequence, batch)
+        self._check(layer, sequence, batch, q)
         nq = q.size // (n_heads * D * batch)
         held = self.lengths[layer, sequence:sequence + batch]
         pos_t, max_keys = None, q_pos0 + nq
@@ -649,7 +649,9 @@ class KVCache8:
                                           q_pos0, pos_t.ptr if pos_t is not None else None, max_keys, scale))
         return out
 
-    def _check(self, layer: int, sequence: int, count: int) -> None:
+    def _check(self, layer: int, sequence: int, count: int, *tensors: Tensor) -> None:
+        if any(t.dev is not self.dev for t in tensors):  # their memory is in the order of another stream
+            raise TensorError(_lib.ERR_DEVICE, "KV cache: a tensor of another device context")
         if not 0 <= layer < self.n_layers:
             raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {layer}, size {self.n_layers}")
         if sequence < 0 or sequence + count > self.max_batch:

@@ -98,3 +98,15 @@ def test_shapes_of_nothing(fake):
         with pytest.raises(_lib.TensorError) as e:
             cache.layer_arrays(0, 0, n)
         assert e.value.code == _lib.ERR_INDEX
+
+
+def test_tensors_of_another_context_are_refused(fake):
+    other = types.SimpleNamespace(**vars(fake))
+    cache = KVCache8(fake, 1, 2, 64, max_seq=100)
+    mine, theirs = _tensor(fake, (1, 2, 64)), _tensor(other, (1, 2, 64))
+    cache.append(0, mine, mine)
+    for call in (lambda: cache.append(0, mine, theirs), lambda: cache.append(0, theirs, mine), lambda: cache.attention(0, theirs, 2)):
+        with pytest.raises(_lib.TensorError) as e:
+            call()
+        assert e.value.code == _lib.ERR_DEVICE
+    assert list(cache.lengths[0]) == [1]
