@@ -111,15 +111,17 @@ __device__ __forceinline__ int turn_key(int lane) { return 4 * ((lane & 7) >> 1)
 __device__ __forceinline__ int turn_d(int lane) { return 8 * (lane >> 4); }
 
 // Rows of K or V (blockIdx.z) of one KV head (blockIdx.y).  A row for each sequence: blockIdx.x is the sequence.  Rows of
-// one sequence: they fall into blocks first .. last; CTA 0 takes the first and the last one, which may both live in the
-// open block's place, and then the length; CTA i > 0 takes block first + i, all of whose rows are new.
+// one sequence: they fall into blocks first .. last, and CTA i takes block first + i, all of whose rows are new if i > 0.
+// Where the first block has rows already and the last one stays open, CTA 0 takes that too, behind the first: both may
+// live in the open block's place.  CTA 0 writes the length.
 //
 // A block that is sealed stays in registers: warp w holds its keys 16 w .. 16 w + 15 in the order in which the codes lie,
 // so that old rows (16 bytes a lane) and codes (512 a warp) are read and written as they are.  K's order takes eight
 // neighbouring values of a row, which is how new rows come too; V's takes four keys of a value, and new rows are turned
-// by ldmatrix.  Bound by the rows' bytes and, for few of them, by the launch: 2048 rows
-// of 32 heads of 128 and their read-back 53.2 -> 25.5 us against a form that went through shared memory value by value,
-// a row for each of 32 sequences of four heads of 64 and theirs 13.8 -> 7.9 (two launches from the host).
+// by ldmatrix.  Rows of an open block go the same way, 16 keys a warp; fewer than four, or behind older ones, one by one.
+// Bound by the rows' bytes and, for few of them, by the launch: 2048 rows of 32 heads of 128 take 13.4 us (3.8 TB/s), 300
+// of them 6.3, 60 3.2 (8.2 and 5.0 with the open block one by one behind the first; the launch alone is 3.1), and 2048
+// with their read-back 22.9 against 53 for a form that went through shared memory value by value.
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
     constexpr int PITCH = D + 8, PIECES = D / 8, C = D / 32;
@@ -240,8 +242,43 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
                     __float2half_rn(s * (float)((int)old[kv ? kv8_v_code<D>(j, d) : kv8_k_code<D>(j, d)] - 128));
             }
         }
-#pragma unroll 4
-        for (int i = j0 * PIECES + tid; i < j1 * PIECES; i += kThreads) {
+        // this warp's 16 keys: by registers where all of them are new and several come (zeros behind them), else one by one
+        const int n0 = j0 > 16 * warp ? j0 : 16 * warp, n1 = j1 < 16 * warp + 16 ? j1 : 16 * warp + 16;
+        if (n0 == 16 * warp && n1 - n0 >= 4) {
+            const int key[2] = {n0 + kv8_key(g), n0 + kv8_key(g + 8)};
+            uint4 *to = reinterpret_cast<uint4 *>(open) + warp * C * 64 + lane;
+            uint4 f[C][2];
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    f[c][h] = make_uint4(0, 0, 0, 0);
+                    if (key[h] < n1) f[c][h] = *reinterpret_cast<const uint4 *>(src + (size_t)(b * kKv8Block + key[h] - pos) * row + c * 32 + t * 8);
+                }
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                f[c][0] = finite8(f[c][0]), f[c][1] = finite8(f[c][1]);
+                if (kv == 0) {
+                    to[c * 64] = make_uint4(f[c][0].x, f[c][0].y, f[c][1].x, f[c][1].y);
+                    to[c * 64 + 32] = make_uint4(f[c][0].z, f[c][0].w, f[c][1].z, f[c][1].w);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) *reinterpret_cast<uint4 *>(xs + key[h] * PITCH + c * 32 + t * 8) = f[c][h];
+                }
+            }
+            if (kv == 0) return;
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    uint32_t r[4];
+                    ldsm4_trans(r, xs + (16 * warp + turn_key(lane)) * PITCH + c * 32 + s * 16 + turn_d(lane));
+                    to[c * 64 + s * 32] = make_uint4(r[0], r[1], r[2], r[3]);
+                }
+            return;
+        }
+        for (int i = n0 * PIECES + lane; i < n1 * PIECES; i += 32) {
             const int j = i / PIECES, d = i % PIECES * 8;
             const uint4 f = finite8(*reinterpret_cast<const uint4 *>(src + (size_t)(b * kKv8Block + j - pos) * row + d));
             if (kv == 0) {
@@ -254,22 +291,20 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
             }
         }
     };
-    if (blockIdx.x > 0 && !batched) {
-        seal(first + blockIdx.x, 0);
+    const int j0 = pos - first * kKv8Block, j1 = pos + m - last * kKv8Block;
+    const int b = first + (batched ? 0 : blockIdx.x);
+    if (b > first && (b < last || j1 == kKv8Block)) {
+        seal(b, 0);
         return;
     }
-    const int j0 = pos - first * kKv8Block, j1 = pos + m - last * kKv8Block;
-    if (last > first || j1 == kKv8Block) {
-        seal(first, j0);
-        if (last > first) {
-            __syncthreads();  // (the open block has been read, and warp_max)
-            if (j1 == kKv8Block) seal(last, 0);
-            else keep(last, 0, j1);
-        }
-    } else {
-        keep(first, j0, j1);
+    if (b == first) {
+        if (last > first || j1 == kKv8Block) seal(first, j0);
+        else __syncthreads();  // (every warp has read the length)
+        if (tid == 0) *length = pos + m;
+        if (j1 == kKv8Block || (last > first && gridDim.x > last - first)) return;  // nothing is open, or another CTA's
+        if (last > first) __syncthreads();                                          // (the open block has been read)
     }
-    if (tid == 0) *length = pos + m;
+    keep(last, last > first ? 0 : j0, j1);
 }
 
 // Block b of a head (K or V), whose cache holds `have` of its rows: the codes (times s) or the open rows of this warp's
@@ -523,8 +558,9 @@ extern "C" int32_t tlc_kvcache8_append(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_
     p.pos = pos_offset;
     p.positions = positions_dev;
     p.status = ctx->dev_status;
-    const int blocks = (pos_offset + m - 1) / kKv8Block - pos_offset / kKv8Block + 1;  // CTA 0 takes two
-    const dim3 grid(batched ? m : blocks > 1 ? blocks - 1 : 1, cache->n_kv_heads, 2);
+    const int blocks = (pos_offset + m - 1) / kKv8Block - pos_offset / kKv8Block + 1;  // (a row for each sequence: not used)
+    const int both = blocks > 1 && pos_offset % kKv8Block > 0 && (pos_offset + m) % kKv8Block > 0;  // first and last, one CTA
+    const dim3 grid(batched ? m : blocks - both, cache->n_kv_heads, 2);
     return launched(ctx, "kvcache8_append",
                     cache->head_dim == 64 ? tlc_launch_pdl(ctx, kv8_append_kernel<64>, grid, dim3(kThreads), 0, p)
                                           : tlc_launch_pdl(ctx, kv8_append_kernel<128>, grid, dim3(kThreads), 0, p));
