@@ -2,7 +2,7 @@
 //
 //   log p(t) = x_t - ln sum e^x,   H = ln sum e^x - sum p x,   over the finite x of a row
 //
-// A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary.  A thread streams 16-byte pieces and
+// A row belongs to a cluster of 1 to 8 CTAs (any number), each with a slice of the vocabulary.  A thread streams 16-byte pieces and
 // keeps a running s = sum 2^y, t = sum 2^y y with y = x log2(e) + c, one fused multiply-add, and c = -m log2(e) in f32
 // for the largest x so far: whatever c is rounded to, log2 p(x) = y - log2 s, so that large logits lose nothing.
 //
@@ -32,12 +32,24 @@ __device__ __forceinline__ float exp2_of(float x) {
     return y;
 }
 
+__device__ __forceinline__ int cluster_rank() {
+    int r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ int cluster_id() {
+    int i;
+    asm("mov.u32 %0, %%clusterid.x;" : "=r"(i));
+    return i;
+}
+
 struct LogprobParams {
     const __half *logits;
     const int *targets;
     float *logprobs, *entropy, *top_logprobs;
     int *top_ids;
-    int rows, vocab, top, cluster, cluster_log2;
+    int rows, vocab, top, cluster;
+    int share;  // 16-byte pieces a CTA
     tlc_dev_status *status;
 };
 struct Sums {
@@ -147,15 +159,16 @@ __device__ __forceinline__ void clean(uint4 w, __half2 none, __half2 (&v)[4]) {
     }
 }
 
-// Without alternatives.  512 x 32000 takes 9.3 us (3.5 TB/s out of the L2 and HBM, 54 % of the copy's rate): 33 MB of
+// Without alternatives.  512 x 32000 takes 9.2 us (3.6 TB/s out of the L2 and HBM, 54 % of the copy's rate): 33 MB of
 // loads with 64 KB in flight an SM, and about 7 instructions a logit.
+template <bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParams p) {
     __shared__ Sums sums[kMaxCluster];
     __shared__ float warp_c[kWarps], warp_s[kWarps], warp_t[kWarps];
-    if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    if (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     tlc_pdl_after_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = blockIdx.x & (p.cluster - 1), row = blockIdx.x >> p.cluster_log2;
+    const int rank = CLUSTER ? cluster_rank() : 0, row = CLUSTER ? cluster_id() : blockIdx.x;
     const __half *x0 = p.logits + (size_t)row * p.vocab;
     Target target = {-1, 0.f};
     Row r;
@@ -165,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
     r.lo = p.logits;
     r.hi = p.logits + (size_t)p.rows * p.vocab;
     r.pieces = (int)(((unsigned)r.ahead + p.vocab + 7) / 8);
-    const int share = (r.pieces + p.cluster - 1) >> p.cluster_log2, first = rank * share, end = min(first + share, r.pieces);
+    const int first = rank * p.share, end = CLUSTER ? min(first + p.share, r.pieces) : r.pieces;
 
     // ---- one pass: the thread's largest value and its sums ----
     Sums run = {INFINITY, 0.f, 0.f};
@@ -263,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
         }
     }
     // ---- the first CTA of the row joins what the others found ----
-    if (p.cluster > 1) {
+    if constexpr (CLUSTER) {
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the row runs
         __syncthreads();
         auto remote = [&](const void *at) {
@@ -313,7 +326,7 @@ __device__ __forceinline__ void ranked(const K *keys, int n, int top, F &&take) 
 // logits are there, 1200 in the exponentials (16384, at 16 a cycle of the SM), the rest between barriers -- bound,
 // candidates, ranks -- and 2000 more in joining the cluster, 1700 in ranking what its CTAs found.  512 threads halve
 // the steps of each against 256 and leave room for a second CTA on the SM.  1 x 32000 with 5 alternatives takes 4.7 us, of
-// which a call's launch is 3.6; 37 x 100003 with 20 12.2.
+// which a call's launch is 3.6; 37 x 100003 with 20 11.2 (seven CTAs a row: all 37 clusters find room at once).
 template <int PIECES>
 __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const LogprobParams p) {
     constexpr int kTurn = kTopThreads * PIECES;  // pieces
@@ -331,14 +344,13 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     tlc_pdl_after_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = blockIdx.x & (p.cluster - 1), row = blockIdx.x >> p.cluster_log2;
+    const int rank = cluster_rank(), row = cluster_id();
     const __half *x0 = p.logits + (size_t)row * p.vocab;
     Target target = {-1, 0.f};
     // The row in 16-byte pieces of memory: the first and the last may reach into other rows, and past the array.
     const int ahead = (int)(((uintptr_t)x0 & 15) >> 1);  // values of the first piece in front of the row
     const __half *base = x0 - ahead;
-    const int pieces = (int)(((unsigned)ahead + p.vocab + 7) / 8), share = (pieces + p.cluster - 1) >> p.cluster_log2;
-    const int first = rank * share, end = min(first + share, pieces);
+    const int pieces = (int)(((unsigned)ahead + p.vocab + 7) / 8), first = rank * p.share, end = min(first + p.share, pieces);
     const int whole_first = ahead > 0, whole_end = (int)(((unsigned)ahead + p.vocab) / 8);  // pieces that are all the row's
 
     if (tid < p.top) best[0][tid] = 0;
@@ -543,7 +555,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const Logpr
     } else {
         // The CTAs' sorted lists: k keys reach the least of their (k / CTAs)-th ones, and no key below it counts.
         unsigned long long *keys = reinterpret_cast<unsigned long long *>(list), least = ~0ull;
-        const int nth = (p.top + p.cluster - 1) >> p.cluster_log2, at = tid % kMaxTop;
+        const int nth = (p.top + p.cluster - 1) / p.cluster, at = tid % kMaxTop;
         for (int i = 0; i < p.cluster; i++) least = min(least, best[i][nth - 1]);
         const unsigned long long key = tid < p.cluster * kMaxTop && at < p.top ? best[tid / kMaxTop][at] : 0;
         if (key > 0 && key >= least) keys[atomicAdd(&found.n, 1)] = key;
@@ -568,25 +580,46 @@ cudaError_t launch_top(tlc_ctx *ctx, cudaLaunchConfig_t &cfg, const LogprobParam
 }
 
 // How many 16-byte pieces a slice has, at most.
-constexpr long long slice_pieces(int vocab, int ctas) { return ((long long)vocab + 14) / 8 / ctas + 1; }
+constexpr int slice_pieces(int vocab, int ctas) { return (int)((((long long)vocab + 14) / 8 + ctas - 1) / ctas); }
 
-// CTAs a row, by cost in microseconds as fitted to calls of 1 to 400 rows of 16000 to 151936 logits with 1, 2, 4 and 8
-// CTAs a row.  A row costs the joining of its CTAs and a CTA's work: a turn of 2048 pieces with alternatives (3.45, with
-// 512 or 1024 pieces 2 or 2.5), 15000 logits a microsecond without.  As many clusters as find an SM for each CTA run at
-// once (4 or 8 CTAs must lie in one part of the chip: a fifth of the SMs stays empty); further ones share SMs and cost
-// 0.8 of that.  With 20 alternatives 36 x 32000 takes 8.9, 6.5, 7.2 and 9.7 us with 1, 2, 4 and 8 CTAs a row, 36 x 100003
-// 27.0, 17.5, 13.8 and 12.2, 148 x 100003 30.3, 25.1, 32.1 and 32.6.
-int ctas_a_row(int sms, int rows, int vocab, bool alternatives) {
-    constexpr double kJoin[2][4] = {{0, 1.1, 1.3, 2.1}, {0, 1.2, 1.4, 1.6}};
+// How many clusters of c CTAs of the kernel with alternatives run at once, two CTAs an SM.
+int resident_clusters(tlc_ctx *ctx, int c) {
+    static int known[64][kMaxCluster + 1] = {};
+    int &n = known[ctx->device & 63][c];
+    if (n > 0) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)c);
+    cfg.blockDim = dim3(kTopThreads);
+    cfg.dynamicSmemBytes = list_size<4>() * sizeof(unsigned);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)c;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, logprob_top_kernel<4>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        clusters = 0;
+    }
+    return n = clusters > 0 ? clusters : 1;
+}
+
+// CTAs a row, by cost in microseconds as fitted to calls of 1 to 400 rows of 16000 to 151936 logits with 1 to 8 CTAs a
+// row.  A row costs the joining of its CTAs and a CTA's work: a turn of 2048 pieces with alternatives (3.45, with 512 or
+// 1024 pieces 2 or 2.5), 15000 logits a microsecond without.  Half of the clusters that run at once find SMs of their own
+// (of more than two CTAs, which lie in one part of the chip, a quarter); all of them take 1.5 times as long, more wait.
+// With 20 alternatives 36 x 32000 takes 9.2, 6.6, 8.5, 7.4, 7.5, 7.7, 8.7 and 9.9 us with 1 to 8 CTAs a row, 36 x 100003
+// 27.3, 17.8, 14.0, 13.9, 13.8, 13.4, 10.1 and 12.3, 148 x 100003 30.4, 25.1, 35.6, 32.5, 37.2, 43.0, 29.8 and 32.8.
+int ctas_a_row(tlc_ctx *ctx, int rows, int vocab, bool alternatives) {
+    constexpr double kJoin[2][kMaxCluster] = {{0, 1.1, 1.2, 1.3, 1.5, 1.7, 1.9, 2.1}, {0, 1.2, 1.3, 1.4, 1.45, 1.5, 1.55, 1.6}};
     int best = 1;
     double least = 1e30;
-    for (int c = 1, i = 0; c <= kMaxCluster; c *= 2, i++) {
-        const long long n = slice_pieces(vocab, c), held = n <= kTopThreads ? 1 : n <= 2 * kTopThreads ? 2 : 4;
+    for (int c = 1; c <= kMaxCluster; c++) {
+        const int n = slice_pieces(vocab, c), held = n <= kTopThreads ? 1 : n <= 2 * kTopThreads ? 2 : 4, all = resident_clusters(ctx, c);
         const double work = alternatives ? (double)((n + held * kTopThreads - 1) / (held * kTopThreads)) * (1.5 + 0.49 * held) : n * 8 / 15000.0;
-        int at_once = (c <= 2 ? sms : sms * 4 / 5) / c;
-        if (at_once < 1) at_once = 1;
-        const int layers = (rows - 1) / at_once + 1;
-        const double cost = kJoin[alternatives][i] + work * (layers == 1 ? 1 : 0.8 * layers);
+        const double times = rows <= all / (c <= 2 ? 2 : 4) ? 1.0 : rows <= all ? 1.5 : (c == 1 ? 0.3 : 0.9) + 1.6 * rows / all;
+        const double cost = kJoin[alternatives][c - 1] + work * times;
         if (cost < least) {
             least = cost;
             best = c;
@@ -620,9 +653,9 @@ extern "C" int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int3
     p.vocab = vocab;
     p.top = top_k;
     p.status = ctx->dev_status;
-    const int c = ctas_a_row(ctx->sm_count, rows, vocab, top_k > 0);
+    const int c = ctas_a_row(ctx, rows, vocab, top_k > 0);
     p.cluster = c;
-    while (1 << p.cluster_log2 < c) p.cluster_log2++;
+    p.share = slice_pieces(vocab, c);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * c));
     cfg.blockDim = dim3(kThreads);
@@ -641,10 +674,9 @@ extern "C" int32_t tlc_token_logprobs(tlc_ctx *ctx, const void *logits_dev, int3
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    const long long pieces = slice_pieces(vocab, c);
-    const cudaError_t le = top_k == 0                  ? cudaLaunchKernelEx(&cfg, logprob_kernel, p)
-                           : pieces <= kTopThreads     ? launch_top<1>(ctx, cfg, p)
-                           : pieces <= 2 * kTopThreads ? launch_top<2>(ctx, cfg, p)
+    const cudaError_t le = top_k == 0                  ? cudaLaunchKernelEx(&cfg, c > 1 ? logprob_kernel<true> : logprob_kernel<false>, p)
+                           : p.share <= kTopThreads     ? launch_top<1>(ctx, cfg, p)
+                           : p.share <= 2 * kTopThreads ? launch_top<2>(ctx, cfg, p)
                                                        : launch_top<4>(ctx, cfg, p);
     if (le != cudaSuccess) {
         cudaGetLastError();
