@@ -206,3 +206,15 @@ def test_far_into_memory(dev, top):
             assert list(host[4][i]) == at and all(abs(g - w) <= tol[0] + 2.0 ** -22 * abs(w) for g, w in zip(host[5][i], b))
     even = np.log(vocab)
     assert abs(float(lp[0]) + even) <= 2.0 ** -18 + 2.0 ** -22 * even and (lp[:-last] == lp[0]).all() and (h[:-last] == h[0]).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(36, 100003), (18, 151937), (48, 151936), (24, 64001), (60, 64000), (20, 32003), (100, 100000)])
+@pytest.mark.parametrize("top", [0, 20])
+def test_many_rows(dev, rows, vocab, top):
+    """Rows shared out over every number of CTAs, and more of them than there is room for at once."""
+    rng = np.random.default_rng(rows + vocab)
+    x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float16)
+    x[rng.random((rows, vocab)) < 0.2] = -np.inf
+    x[::5, vocab // 3:] = -np.inf                     # slices with nothing in them
+    check(dev, x, rng.integers(0, vocab, rows), top)
+    dev.synchronize()
