@@ -18,10 +18,12 @@
 // (distributed shared memory); of several clusters the last one (a ticket for each share of the rows) joins what all have
 // left in the cache's workspace.
 //
-// Many sequences: bound by HBM while all warps have blocks (32 sequences of about 600 keys, 32 heads of 128: 34 us, 157 MB
-// at 0.70 of the copy's rate; the tensor pipe is 15 % busy).  One sequence: by latency, 1.0 us a block and warp, and the
-// merge (65000 keys, 4 KV heads of 64: 14 us; 512 keys 5.5, of which a call's launch is 3.6).
+// Many sequences: bound by HBM while all warps have blocks (32 sequences of about 600 keys, 32 heads of 128: 33 us, 157 MB
+// at 0.72 of the copy's rate; the tensor pipe is 15 % busy).  One sequence: by latency, 1.0 us a block and warp, and the
+// merge (65000 keys, 4 KV heads of 64: 12.5 us; 512 keys 5.5, of which a call's launch is 3.6).
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "tlc_kv8.h"
 
@@ -31,7 +33,10 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr float kShift = 12.f;        // P is held times 2^12
 constexpr float kUp = 16777216.f;     // the codes' 2^24
 constexpr float kLog2e = 1.4426950408889634f;
-template <int D> constexpr int stages() { return D == 128 ? 3 : 6; }  // of 64 * D bytes (K or V of a block) per warp
+// CTAs an SM.  Rows of 64 values, up to eight rows an item: four, at 128 registers and half the ring, as a block is more
+// latency than bytes (65000 keys, 4 KV heads: 13.7 -> 12.4 us; 64 sequences of 1500: 11.1 -> 10.4).
+constexpr int places(int D, int nt) { return D == 64 && nt == 1 ? 4 : 2; }
+template <int D, int NT> constexpr int stages() { return D == 64 && NT == 2 ? 6 : 3; }  // of 64 * D bytes (K or V of a block) per warp
 
 struct Params {
     const __half *q;  // [batch * I, H, D]
@@ -77,8 +82,8 @@ __device__ __forceinline__ uint32_t low2(uint32_t w) { return __byte_perm(w, 0, 
 __device__ __forceinline__ uint32_t high2(uint32_t w) { return __byte_perm(w, 0, 0x4342); }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
-    constexpr int ROWS = 8 * NT, STAGE = kKv8Block * D, ST = stages<D>(), LOADS = STAGE / 512, PITCH = D + 4;
+__global__ void __launch_bounds__(kThreads, places(D, NT)) attention8_kernel(const Params p) {
+    constexpr int ROWS = 8 * NT, STAGE = kKv8Block * D, ST = stages<D, NT>(), LOADS = STAGE / 512, PITCH = D + 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];  // in a cluster: of the CTA in [0], for its peers
     __shared__ int sm_last;
@@ -602,11 +607,11 @@ __global__ void __launch_bounds__(kThreads) attention8_kernel(const Params p) {
 
 template <int D, int NT>
 int32_t launch(tlc_ctx *ctx, const Params &p) {
-    constexpr size_t smem = (size_t)kWarps * stages<D>() * kKv8Block * D;
+    constexpr size_t smem = (size_t)kWarps * stages<D, NT>() * kKv8Block * D;
     int ctas = p.items * p.nsplit;
-    if (p.nsplit == 1) {  // both places of every SM, as far as items go
+    if (p.nsplit == 1) {  // all places of every SM, as far as items go
         const int groups = kWarps / p.warps, least = (p.items + groups - 1) / groups;
-        ctas = p.items < 2 * ctx->sm_count ? p.items : 2 * ctx->sm_count;
+        ctas = std::min(p.items, places(D, NT) * ctx->sm_count);
         if (ctas < least) ctas = least;
     }
     const dim3 grid((unsigned)ctas);
@@ -648,19 +653,26 @@ int32_t launch(tlc_ctx *ctx, const Params &p) {
 // Warps that share an item of `units` blocks -- 1, 2, 4, or four in each of 2, 4, 8 or a multiple of eight CTAs: the
 // fewest microseconds of
 //   blocks of a warp x (the larger of a block's latency and its share of the SM, 44 KB/us for its warps),
-// as often as the SM's eight warps have to be filled, and the merge, in shared memory, in a cluster, or of clusters.
+// as often as the SM's warps have to be filled, and the merge, in shared memory, in a cluster, or of clusters.  (Clusters of
+// eight lie in one part of the chip: beyond two for nine SMs they leave some SMs with more CTAs than others.)
+// One query, 32 heads on four of 64, behind 40000 positions takes 14.2 us with 64 warps to a KV head, 11.9 with 128, 12.5
+// with 256, 16.2 with 576; behind 130000 30, 22, 17 and 21.
 // Sixteen queries behind 1000 positions, 32 heads of 128: one warp 28.5 us, two 19.8, four 12.8, sixteen 11.8; 192
 // queries: 49.2, 31.9, 35.6, 68.
 double share_out(const tlc_ctx *ctx, int D, int nt, int units, Params &p) {
     const double latency = D == 64 ? nt == 1 ? 0.85 : 1.05 : nt == 1 ? 1.2 : 1.6, share = kKv8Block * D * 2 / 44e3;
+    const int warps = kWarps * places(D, nt);  // of an SM
     double best = 1e30;
     for (int w = 1; w <= 4 * kKv8MaxCtas; w = w < 32 ? 2 * w : w + 32) {
         const int nsplit = w <= kWarps ? 1 : w / kWarps, cluster = nsplit < 8 ? nsplit : 8;
         if (w > 1 && w >= 2 * units) break;  // (fewer would do)
         if (nsplit > 8 && ((long long)p.items * nsplit > kKv8MaxCtas || p.items * 8 > kKv8Tickets)) break;
-        const long long per_sm = ((long long)p.items * w + ctx->sm_count - 1) / ctx->sm_count, rounds = (per_sm + 7) / 8;
-        const double at_once = (double)(per_sm < 8 ? per_sm : 8), block = latency > at_once * share ? latency : at_once * share;
-        const double t = (double)rounds * ((units + w - 1) / w) * block + (w == 1 ? 0.0 : w <= kWarps ? 0.7 : nsplit <= 8 ? 1.5 : 3.5);
+        const long long clusters = (long long)p.items * (nsplit / 8), layer = ctx->sm_count / 9 > 0 ? ctx->sm_count / 9 : 1;
+        const long long per_sm = nsplit > 8 && clusters > 2 * layer ? kWarps * ((clusters + layer - 1) / layer)
+                                                                    : ((long long)p.items * w + ctx->sm_count - 1) / ctx->sm_count;
+        const long long rounds = (per_sm + warps - 1) / warps;
+        const double at_once = (double)(per_sm < warps ? per_sm : warps), block = latency > at_once * share ? latency : at_once * share;
+        const double t = (double)rounds * ((units + w - 1) / w) * block + (w == 1 ? 0.0 : w <= kWarps ? 0.7 : nsplit <= 8 ? 1.5 : 3.0 + 0.12 * (nsplit / 8));
         if (t < best) {
             best = t;
             p.warps = w < kWarps ? w : kWarps;
