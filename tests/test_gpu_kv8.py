@@ -48,9 +48,10 @@ def check_attention(got, q, k, v, pos0, scale=None):
     output to f16 (2^-11 of itself, or half the smallest subnormal).  In f32: a score is a sum of D products of q with
     codes + 128 (at most 255) in steps of 16, each step good to 2^-23 of what has been added up -- below
     (D / 16 + 4) 2^-23 * 255 / 127 * sum |q| max|k| scale -- and e^x itself to 2^-21; both act on p.  The second product
-    adds p (code + 128) to -128 sum p: sum p comes from six additions and five more across lanes, four steps follow,
-    each good to 2^-23 of at most 255 sum p, and a code is worth max|v| / 127 -- below 16 * 2^-23 * 255 / 127 * max|v|
-    whatever the values that count (they may all be zero)."""
+    adds p (code + 128), all of one sign, to be taken off as 128 sum p: in a step of 16 the products are aligned to the
+    largest and cut, so that each of a block's 64 may lose 2^-23 of at most 255 sum p, and so may each of eleven additions
+    of sum p and the four that join them.  A code is worth max|v| / 127 -- below 80 * 2^-23 * 255 / 127 * max|v| whatever the
+    values that count (they may all be zero)."""
     I, H, D = q.shape
     G = H // k.shape[1]
     scale = D ** -0.5 if scale is None else scale
@@ -64,7 +65,7 @@ def check_attention(got, q, k, v, pos0, scale=None):
         want, size = p @ vh, p @ np.abs(vh)
         score = (D / 16 + 4) * 2.0 ** -23 * 255 / 127 * abs(scale) * np.abs(qh).sum(1, keepdims=True) * np.abs(kh).max() + 2.0 ** -21
         tol = 2.0 ** -11 * np.abs(want) + (2 * 2.0 ** -11 + 2 * score) * size + 2.0 ** -25
-        tol += 16 * 2.0 ** -23 * 255 / 127 * np.abs(vh).max()
+        tol += 80 * 2.0 ** -23 * 255 / 127 * np.abs(vh).max()
         err = np.abs(got[:, h].astype(np.float64) - want)
         assert np.isfinite(got[:, h]).all()
         worst = max(worst, float((err / tol).max()))
@@ -481,3 +482,23 @@ def test_far_into_memory(dev):
     check_attention(token[1:], q[-1:], exact_values(k), exact_values(v), T - 1)
     assert not token[0].any()
     dev.synchronize()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("I", [1, 8, 400])
+def test_scales_apart(dev, D, I):
+    """Blocks of very different scale, and in a block of large values one row of tiny ones that most of P falls on."""
+    from tensorlogic_b200.api import KVCache8
+    H, Hkv, T = 4, 2, 640
+    k, v = (a.astype(np.float32) for a in rows(7, T, Hkv, D))
+    for a in (k, v):
+        a[:64] *= 30
+        a[64:320] *= 1e-3
+    q = queries(7, I, H, D)
+    k[5] = 8 * q[0].reshape(Hkv, H // Hkv, D)[:, 0] / np.sqrt(D) * 8
+    v[5] = 1e-4
+    k, v = k.astype(np.float16), v.astype(np.float16)
+    cache = KVCache8(dev, 1, Hkv, D, max_seq=T)
+    cache.append(0, dev.tensor(k), dev.tensor(v))
+    got = cache.attention(0, dev.tensor(q), H, q_pos0=T - I).numpy()
+    check_attention(got, q, exact_values(k), exact_values(v), T - I)
