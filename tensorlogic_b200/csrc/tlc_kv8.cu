@@ -416,7 +416,9 @@ __global__ void __launch_bounds__(kThreads) kv8_widen_kernel(const WidenParams p
     }
     if (tid == 0) {
         float *to = reinterpret_cast<float *>(p.factors + (size_t)hk * p.c.n_blocks + b);
-        const float w = s > 0.f ? s : 1.f;  // (a block of zeros: any factor but zero)
+        // A block of zeros counts for nothing in P.V, so what it is given must not lift the running maximum, which log2 of
+        // the factor is part of, over other blocks: 2^-31, below the smallest scale there is (2^-24 / 127).
+        const float w = s > 0.f ? s : 0x1p-31f;
         if (kv == 0) to[0] = s;
         else to[1] = log2f(w), to[2] = 1.f / w;
     }
