@@ -62,6 +62,9 @@ __device__ __forceinline__ void tma_load_3d_el(uint32_t dst, const void *map, in
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(el)
         : "memory");
 }
+// An average of what the cache holds lies within f16.  Its sum of P is of the values before they were rounded, so that
+// values next to 65504 could come out up to 2^-11 above it, an infinity.  (NaN stays.)
+__device__ __forceinline__ __half2 in_range(__half2 v) { return __hmax2_nan(__hmin2_nan(v, __float2half2_rn(65504.f)), __float2half2_rn(-65504.f)); }
 // Columns of this thread's lane.  The load is waited for by tmem_ld_wait, which the registers pass through: nothing
 // that uses them can be moved in front of it.
 __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t (&r)[32]) {
@@ -318,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     __align__(16) __half2 h[4];
 #pragma unroll
                     for (int i = 0; i < 8; i += 2)
-                        h[i / 2] = __floats2half2_rn(__uint_as_float(o[e + i]) * inv, __uint_as_float(o[e + i + 1]) * inv);
+                        h[i / 2] = in_range(__floats2half2_rn(__uint_as_float(o[e + i]) * inv, __uint_as_float(o[e + i + 1]) * inv));
                     *reinterpret_cast<uint4 *>(out + c + e) = *reinterpret_cast<const uint4 *>(h);
                 }
             }

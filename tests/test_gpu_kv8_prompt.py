@@ -48,3 +48,20 @@ def test_nothing_but_zeros(dev):
     cache.append(0, dev.tensor(k), dev.tensor(np.zeros((T, Hkv, D))))
     assert not prompt(dev, cache, q, H).any()
     dev.synchronize()
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(32, 4, 64), (8, 2, 128)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_largest_values(dev, H, Hkv, D, sign):
+    """Values that are all the largest f16: so is their average, whatever P is rounded to."""
+    from tensorlogic_b200.api import KVCache8
+    T = 1000
+    rng = np.random.default_rng(D)
+    k = np.zeros((T, Hkv, D), np.float16)
+    k[64:] = rng.standard_normal((Hkv, D)) * 0.01  # (one score in front, another behind: P of the latter rounds as one)
+    v = np.full((T, Hkv, D), sign * 65504, np.float16)
+    q = rng.standard_normal((T, H, D)).astype(np.float16)
+    cache = KVCache8(dev, 1, Hkv, D, max_seq=T)
+    cache.append(0, dev.tensor(k), dev.tensor(v))
+    check_attention(prompt(dev, cache, q, H), q, exact_values(k), exact_values(v), 0)
+    dev.synchronize()
