@@ -123,7 +123,9 @@ TLC_API int32_t tlc_destroy(tlc_ctx *ctx);
  *   "gemm_pg"     (0, 1 or 2) accepted and without effect: one group of weight producers a CTA;
  *   "q6k_resident" Q6_K tensors stay quantized in HBM (1, default) or become f16 at upload (0);
  *   "attn_wide"   decode attention of one sequence with at most four KV heads over a long
- *                 context runs on clusters of sixteen key splits (1) or eight (0, default: no slower).
+ *                 context runs on clusters of sixteen key splits (1) or eight (0, default: no slower);
+ *   "attn8_tc"    prompts over the 8-bit cache run on the tensor-memory kernel wherever it can take them
+ *                 (1), never (2), or where it is the faster one by its cost (0, default).
  * Unknown names fail with TLC_ERR_INVALID_OPERATION. */
 TLC_API int32_t tlc_set_option(tlc_ctx *ctx, const char *name, int64_t value);
 /* Failure-detection self-test.  Enqueues a kernel whose device-side wait can never be

@@ -737,7 +737,8 @@ extern "C" int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
     TLC_REQUIRE(items <= INT_MAX, TLC_ERR_INVALID_DIMENSION, "attention8: %d sequences of %d queries", batch, n_queries);
     p.items = (int)items;
     const double t = share_out(ctx, D, nt, (int)((T + kKv8Block - 1) / kKv8Block), p);
-    if (n_queries > 1 && G <= 128 && batch * tcgen05_us(ctx, D, Hkv, G, n_queries, q_pos0) < t && kv8_image(ctx, cache)) {
+    const bool tc = ctx->attn8_tc == 0 ? batch * tcgen05_us(ctx, D, Hkv, G, n_queries, q_pos0) < t : ctx->attn8_tc == 1;
+    if (n_queries > 1 && G <= 128 && tc && kv8_image(ctx, cache)) {
         // (a sequence at a time; without room for its image the kernel below does it, more slowly)
         for (int b = 0; b < batch; b++) {
             const size_t at = (size_t)b * n_queries * n_heads * D;

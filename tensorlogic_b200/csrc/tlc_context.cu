@@ -133,7 +133,10 @@ extern "C" int32_t tlc_set_option(tlc_ctx *ctx, const char *name, int64_t value)
         ctx->pdl_mode = (int)value;
     } else if (n == "attn_wide")
         ctx->attn_wide = (int)value;
-    else if (n == "host_graph")
+    else if (n == "attn8_tc") {
+        TLC_REQUIRE(value >= 0 && value <= 2, TLC_ERR_INVALID_OPERATION, "set_option: attn8_tc must be 0, 1 or 2");
+        ctx->attn8_tc = (int)value;
+    } else if (n == "host_graph")
         ctx->host_graph = value != 0;
     else if (n == "host_poll")
         ctx->host_poll = value != 0;

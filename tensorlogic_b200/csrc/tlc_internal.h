@@ -75,6 +75,7 @@ struct tlc_ctx {
     // key splits (a non-portable cluster size) instead of eight.  Off: measured no faster (one
     // rank's share of the 70B-shape decode at TP8, 2048 keys: 3.79 ms per step against 3.73 ms).
     int attn_wide = 0;
+    int attn8_tc = 0;
     bool host_graph = true;  // decode_host: ids up, the step, results down as ONE graph launch
     bool host_poll = true;   // ... and the host watches the pinned result words instead of a stream sync
     // How long a device-side wait (mbarrier, peer flag) may last before the kernel gives up,
