@@ -409,13 +409,13 @@ def token_logprobs(logits: Tensor, tokens=None, top_k: int = 0):
         raise TensorError(_lib.ERR_INVALID_DIMENSION, f"token_logprobs: bad shape {list(logits.shape)}")
     rows, ids_t = logits.size // vocab, None
     if tokens is not None:
-        ids = np.ascontiguousarray(np.atleast_1d(tokens), dtype=np.int32).reshape(-1)
+        ids = _whole(tokens)
         if ids.size != rows:
             raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"token_logprobs: {ids.size} tokens for {rows} rows")
         wrong = (ids < -1) | (ids >= vocab)
         if wrong.any():
             raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {ids[wrong][0]}, size {vocab}")
-        ids_t = _upload_i32(dev, ids)
+        ids_t = _upload_i32(dev, ids.astype(np.int32))
     if not 0 <= top_k <= 32:
         raise TensorError(_lib.ERR_INVALID_OPERATION, f"token_logprobs: top_k {top_k} outside 0 .. 32")
     per = 2 + 2 * top_k  # 4-byte words a row
@@ -449,6 +449,20 @@ def _upload_i32(dev: Device, a: np.ndarray) -> Tensor:
     check(dev.lib.tlc_upload(dev.handle, t.ptr, a.ctypes.data, a.nbytes))
     dev.synchronize()
     return t
+
+
+def _whole(values) -> np.ndarray:
+    """Positions or token ids in 64 bits, whatever holds them: their range is checked on what the caller gave, not on what
+    32 bits leave of it."""
+    a = np.asarray(values).reshape(-1)
+    try:
+        with np.errstate(invalid="ignore"):
+            whole = a.astype(np.int64)
+    except OverflowError:
+        raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: {a[:8]} in 64 bits") from None
+    if a.dtype.kind != "i" and not np.array_equal(whole, a):
+        raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {a[whole != a][0]} is no whole number in 64 bits")
+    return whole
 
 
 # -- fused entry points --------------------------------------------------------
@@ -595,13 +609,13 @@ class KVCache8:
                 raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {at}, size {held[0]}")
         else:
             at = 0
-            pos = np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
+            pos = np.maximum(_whole(positions), -1)  # (any negative one: none)
             if pos.size != m:
                 raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"KV cache: {pos.size} positions for {m} rows")
             wrong = (pos > held[:m]) | (pos >= self.max_seq)
             if wrong.any():
                 raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {pos[wrong][0]}, size {held[:m][wrong][0]}")
-            pos_t = _upload_i32(self.dev, pos)
+            pos_t = _upload_i32(self.dev, pos.astype(np.int32))
         check(self.dev.lib.tlc_kvcache8_append(self.dev.handle, self.handle, layer, k.ptr, v.ptr, m, sequence, at,
                                                pos_t.ptr if pos_t is not None else None))
         if positions is None:
@@ -636,12 +650,12 @@ class KVCache8:
             if wrong.any():
                 raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {q_pos0 + nq - 1}, size {held[wrong][0]}")
         else:
-            pos = np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
+            pos = np.maximum(_whole(positions), -1)  # (any negative one: none)
             if pos.size != batch:
                 raise TensorError(_lib.ERR_SHAPE_MISMATCH, f"attention: {pos.size} positions for {batch} sequences")
             if (pos >= held).any():
                 raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {pos[pos >= held][0]}, size {held[pos >= held][0]}")
-            pos_t = _upload_i32(self.dev, pos)
+            pos_t = _upload_i32(self.dev, pos.astype(np.int32))
             max_keys = max(int(pos.max()) + 1, 1)
         out = Tensor._new(self.dev, q.shape, q.size)
         scale = 1.0 / math.sqrt(D) if scale is None else scale

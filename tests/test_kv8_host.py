@@ -110,3 +110,52 @@ def test_tensors_of_another_context_are_refused(fake):
             call()
         assert e.value.code == _lib.ERR_DEVICE
     assert list(cache.lengths[0]) == [1]
+
+
+@pytest.mark.parametrize("wrong", [2**32, 2**32 + 5, 2**63 - 1, -2**32 + 5, 2**64, 5.5, np.nan, np.uint64(2**63 + 5), np.float32(2**33)])
+def test_indices_are_checked_before_they_are_cut(fake, wrong):
+    """A position or a token that 32 bits do not hold is out of bounds (or, negative, no position), not what is left of it."""
+    cache = KVCache8(fake, 1, 2, 64, max_seq=100, max_batch=2)
+    one = lambda n: _tensor(fake, (n, 2, 64))  # noqa: E731
+    cache.append(0, one(40), one(40), sequence=0)
+    cache.append(0, one(40), one(40), sequence=1)
+    made = len(fake.lib.calls)
+    none = wrong == -2**32 + 5  # any negative position: no row
+    for both in (np.array([40, wrong]), [40, wrong]):
+        for call in (lambda: cache.append(0, one(2), one(2), positions=both),
+                     lambda: cache.attention(0, one(2), 2, batch=2, positions=np.asarray(both) - 1)):
+            if not none:
+                with pytest.raises(_lib.TensorError) as e:
+                    call()
+                assert e.value.code == _lib.ERR_INDEX
+    with pytest.raises(_lib.TensorError) as e:
+        token_logprobs(_tensor(fake, (2, 10)), [3, wrong])
+    assert e.value.code == _lib.ERR_INDEX
+    assert len(fake.lib.calls) == made and list(cache.lengths[0]) == [40, 40]
+    if none:
+        cache.append(0, one(2), one(2), positions=np.array([40, wrong]))
+        assert list(cache.lengths[0]) == [41, 40]
+
+
+def test_negative_positions_stay_negative(fake, monkeypatch):
+    """What reaches the GPU for a position far below zero is below zero too."""
+    from tensorlogic_b200 import api
+    sent = []
+    monkeypatch.setattr(api, "_upload_i32", lambda dev, a: sent.append(a) or types.SimpleNamespace(ptr=4096))
+    cache = KVCache8(fake, 1, 2, 64, max_seq=100, max_batch=3)
+    three = _tensor(fake, (3, 2, 64))
+    cache.append(0, three, three, positions=np.array([0, -2**32 + 5, -1]))
+    cache.attention(0, three, 2, batch=3, positions=np.array([0, -2**32 + 5, -2**63]))
+    cache.append(0, three, three, positions=np.array([1.0, -1.0, -1.0]))  # whole numbers, whatever holds them
+    assert [a.dtype for a in sent] == [np.int32] * 3
+    assert [list(a) for a in sent] == [[0, -1, -1], [0, -1, -1], [1, -1, -1]]
+    assert list(cache.lengths[0]) == [2, 0, 0]
+
+
+def test_tokens_of_any_integer_type(fake, monkeypatch):
+    from tensorlogic_b200 import api
+    sent = []
+    monkeypatch.setattr(api, "_upload_i32", lambda dev, a: sent.append(a) or types.SimpleNamespace(ptr=4096))
+    for t in (np.int8, np.uint8, np.int64, np.uint64):
+        token_logprobs(_tensor(fake, (2, 10)), np.array([3, 9], t))
+    assert all(a.dtype == np.int32 and list(a) == [3, 9] for a in sent) and len(sent) == 4
