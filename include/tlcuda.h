@@ -432,7 +432,9 @@ TLC_API int32_t tlc_attention_decode_static_status(void *stream, int32_t *clampe
  * values, K and V apart.  The rows of a block that is not full yet are held in f16 as they came, so a value is
  * rounded once and does not depend on how many rows came with each call.  The cache holds finite values: NaN
  * becomes zero, an infinity +-65504.  head_dim is 64 or 128.  It keeps, per layer and sequence, how many
- * rows it holds, on the device.  A cache belongs to the context that made it (others are refused). */
+ * rows it holds, on the device.  A cache belongs to the context that made it (others are refused).
+ * Bytes: 2 * n_kv_heads * head_dim * max_seq for each layer and sequence, twice that once for the whole cache (what the
+ * tensor-memory kernel reads a prompt's sequence from), and the open blocks. */
 typedef struct tlc_kvcache8 tlc_kvcache8;
 TLC_API int32_t tlc_kvcache8_create(tlc_ctx *ctx, int32_t n_layers, int32_t max_batch, int32_t max_seq,
                                     int32_t n_kv_heads, int32_t head_dim, tlc_kvcache8 **out);
@@ -456,10 +458,8 @@ TLC_API int32_t tlc_kvcache8_rows(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
  * heads per KV head; q and out 16-byte aligned.  Scores, softmax and sums are f32.  With positions_dev a
  * negative position marks an idle slot, whose output rows are zeros.  A query at a position whose key the cache
  * does not hold (or at or past max_keys) sees the keys there are, and the next tlc_synchronize reports
- * TLC_ERR_INDEX.  Allocates nothing, except on the first prompt long enough for the tensor-memory kernel (an
- * f16 image of one sequence and layer); in a stream capture, and where there is no room for it, such a prompt
- * runs on the other kernel, several times slower: make the first one before a capture.  Calls over one cache
- * share its workspace and run one after the other, replays of captured ones included. */
+ * TLC_ERR_INDEX.  Allocates nothing.  Calls over one cache share its workspace and run one after the other, replays
+ * of captured ones included. */
 TLC_API int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t layer, const void *q_dev,
                                void *out_dev, int32_t batch, int32_t n_queries, int32_t n_heads,
                                int32_t sequence, int32_t q_pos0, const int32_t *positions_dev,

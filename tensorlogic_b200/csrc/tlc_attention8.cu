@@ -738,9 +738,8 @@ extern "C" int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
     p.items = (int)items;
     const double t = share_out(ctx, D, nt, (int)((T + kKv8Block - 1) / kKv8Block), p);
     const bool tc = ctx->attn8_tc == 0 ? batch * tcgen05_us(ctx, D, Hkv, G, n_queries, q_pos0) < t : ctx->attn8_tc == 1;
-    if (n_queries > 1 && G <= 128 && tc && kv8_image(ctx, cache)) {
-        // (a sequence at a time; without room for its image the kernel below does it, more slowly)
-        for (int b = 0; b < batch; b++) {
+    if (n_queries > 1 && G <= 128 && tc) {
+        for (int b = 0; b < batch; b++) {  // through one image, a sequence at a time
             const size_t at = (size_t)b * n_queries * n_heads * D;
             if (int32_t rc = kv8_attention_tc(ctx, cache, layer, sequence + b, static_cast<const __half *>(q_dev) + at,
                                               static_cast<__half *>(out_dev) + at, n_queries, n_heads, q_pos0, scale))

@@ -357,21 +357,6 @@ int32_t launch(tlc_ctx *ctx, const Params &p, const CUtensorMap &q, const CUtens
 
 }  // namespace
 
-bool kv8_image(tlc_ctx *ctx, tlc_kvcache8 *cache) {
-    if (cache->wide) return true;
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(ctx->stream, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone) {
-        const size_t rows = (size_t)cache->n_kv_heads * cache->n_blocks * kKv8Block;
-        cudaError_t e = cudaSuccess;
-        if (!cache->factors) e = cudaMalloc(&cache->factors, (size_t)cache->n_kv_heads * cache->n_blocks * sizeof(float4));
-        if (e == cudaSuccess) e = cudaMalloc(&cache->wide, 2 * rows * cache->head_dim * sizeof(__half));
-        if (e == cudaSuccess) return true;
-        cache->wide = nullptr;
-    }
-    cudaGetLastError();
-    return false;
-}
-
 int32_t kv8_attention_tc(tlc_ctx *ctx, tlc_kvcache8 *cache, int layer, int sequence, const __half *q, __half *out, int I, int H,
                          int pos0, float scale) {
     const uint64_t D = cache->head_dim, Hkv = cache->n_kv_heads, rows = (uint64_t)cache->n_blocks * kKv8Block;

@@ -501,6 +501,7 @@ extern "C" int32_t tlc_kvcache8_create(tlc_ctx *ctx, int32_t n_layers, int32_t m
     c->n_kv_heads = n_kv_heads;
     c->head_dim = head_dim;
     c->n_blocks = (int)blocks;
+    const size_t blocks_of_one = (size_t)n_kv_heads * blocks, wide = blocks_of_one * 2 * block * sizeof(__half);  // a sequence and layer
     const size_t open = heads * 2 * block * sizeof(__half), lengths = heads * 2 * sizeof(int), tickets = kKv8Tickets * sizeof(int);
     cudaError_t e = cudaMalloc(&c->codes, codes);
     if (e == cudaSuccess) e = cudaMalloc(&c->scales, heads * blocks * 2 * sizeof(float));
@@ -508,6 +509,8 @@ extern "C" int32_t tlc_kvcache8_create(tlc_ctx *ctx, int32_t n_layers, int32_t m
     if (e == cudaSuccess) e = cudaMalloc(&c->lengths, lengths);
     if (e == cudaSuccess) e = cudaMalloc(&c->tickets, tickets);
     if (e == cudaSuccess) e = cudaMalloc(&c->partial, (size_t)kKv8MaxCtas * kKv8MaxRows * (head_dim + 2) * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&c->wide, wide);
+    if (e == cudaSuccess) e = cudaMalloc(&c->factors, blocks_of_one * sizeof(float4));
     // Codes and scales are read only after they have been written; rows of an open block past its length are
     // multiplied by zero, and have to be finite for that.
     if (e == cudaSuccess) e = cudaMemsetAsync(c->open, 0, open, ctx->stream);
@@ -516,7 +519,7 @@ extern "C" int32_t tlc_kvcache8_create(tlc_ctx *ctx, int32_t n_layers, int32_t m
     if (e != cudaSuccess) {
         cudaGetLastError();
         tlc_kvcache8_destroy(c);
-        return tlc_fail(TLC_ERR_ALLOCATION, "8-bit KV cache allocation of %zu bytes failed: %s", codes + open, cudaGetErrorString(e));
+        return tlc_fail(TLC_ERR_ALLOCATION, "8-bit KV cache allocation of %zu bytes failed: %s", codes + open + wide, cudaGetErrorString(e));
     }
     *out = c;
     return TLC_OK;

@@ -35,8 +35,8 @@ struct tlc_kvcache8 {
     int *lengths;     // [layer][sequence][kv head][K, V]: rows held (a copy for each CTA that appends)
     float *partial;   // shared keys: [CTA][row][D + 2]
     int *tickets;     // zero between launches
-    // Made on first use by a long prompt: the blocks of one layer and sequence as f16 rows [K, V][kv head][position][D],
-    // and per block what they count (kv8_widen).
+    // For long prompts: the blocks of one layer and sequence as f16 rows [K, V][kv head][position][D], and per block what
+    // they count (kv8_widen).  Made with the cache, so that no prompt allocates, in a stream capture or out of it.
     __half *wide;
     float4 *factors;
     size_t heads() const { return (size_t)max_batch * n_kv_heads; }  // of a layer
@@ -60,8 +60,6 @@ int32_t kv8_check(tlc_ctx *ctx, const tlc_kvcache8 *cache, const char *what, int
 
 // Fills wide and factors with the first `blocks` blocks of a sequence.
 int32_t kv8_widen(tlc_ctx *ctx, tlc_kvcache8 *cache, int layer, int sequence, int blocks);
-// Makes room for them, where there is none yet: not while the stream is being captured, and not if there is no memory.
-bool kv8_image(tlc_ctx *ctx, tlc_kvcache8 *cache);
 // Attention of a prompt over that image on the 5th-generation tensor cores (tlc_attention8_tc.cu).
 int32_t kv8_attention_tc(tlc_ctx *ctx, tlc_kvcache8 *cache, int layer, int sequence, const __half *q, __half *out, int I, int H,
                          int pos0, float scale);

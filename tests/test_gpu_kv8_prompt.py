@@ -262,3 +262,35 @@ def test_which_kernel_runs(dev):
             dev.set_option("attn8_tc", wrong)
         assert e.value.code == _lib.ERR_INVALID_OPERATION
     dev.synchronize()
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(32, 4, 64), (8, 2, 128)])
+def test_first_prompt_in_a_capture(dev, H, Hkv, D):
+    """A cache's first long prompt, in a graph: it runs on the kernel that it runs on outside of one, and allocates nothing."""
+    import torch
+    from tensorlogic_b200 import _lib
+    from tensorlogic_b200.api import KVCache8
+    I = 900
+    k, v = rows(2, I, Hkv, D)
+    q = queries(2, I, H, D)
+    cache = KVCache8(dev, 1, Hkv, D, max_seq=1000, max_batch=2)
+    cache.append(0, dev.tensor(k), dev.tensor(v), sequence=1)
+    tq, out = torch.tensor(q, device="cuda"), torch.zeros(I, H, D, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    dev.synchronize()
+    before = dev.launch_count
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.ExternalStream(dev.stream)):
+        _lib.check(dev.lib.tlc_attention8(dev.handle, cache.handle, 0, tq.data_ptr(), out.data_ptr(), 1, I, H, 1, 0, None, 0, D ** -0.5))
+    assert dev.launch_count - before == 2
+    g.replay()
+    torch.cuda.synchronize()
+    got = out.cpu().numpy()
+    check_attention(got, q, exact_values(k), exact_values(v), 0)
+    out.zero_()
+    torch.cuda.synchronize()
+    free = dev.mem_info()[0]
+    _lib.check(dev.lib.tlc_attention8(dev.handle, cache.handle, 0, tq.data_ptr(), out.data_ptr(), 1, I, H, 1, 0, None, 0, D ** -0.5))
+    dev.synchronize()
+    assert dev.mem_info()[0] == free
+    assert same(out.cpu().numpy(), got)
