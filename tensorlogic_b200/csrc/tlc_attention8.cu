@@ -50,7 +50,7 @@ struct Params {
     int items, row_tiles;
     int warps, nsplit;  // warps of a CTA per item (1, 2, 4), CTAs per item (more than one: of four warps)
     int cluster;        // CTAs of a cluster: nsplit if that is 1, 2, 4 or 8, else 8
-    float *partial;  // of several clusters: [cluster][row][2], then [cluster][row][D]
+    float *partial;  // of several clusters: [item][cluster][row][2], then [item][cluster][row][D]
     int *tickets;
     tlc_dev_status *status;
 };
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, places(D, NT)) attention8_kernel(con
     cluster_barrier();
     const int n_clusters = p.nsplit / p.cluster;
     const size_t slot = (size_t)item * n_clusters + split / p.cluster;
-    float *part_ml = p.partial, *part_o = p.partial + (size_t)kKv8MaxCtas * kKv8MaxRows * 2;
+    float *part_ml = p.partial, *part_o = p.partial + (size_t)kKv8MaxParts * kKv8MaxRows * 2;
     for (int i = tid; i < per * Q; i += kThreads) {
         const int r = per * rank + i / Q, q = i % Q;
         float m[8], l[8];

@@ -508,7 +508,7 @@ extern "C" int32_t tlc_kvcache8_create(tlc_ctx *ctx, int32_t n_layers, int32_t m
     if (e == cudaSuccess) e = cudaMalloc(&c->open, open);
     if (e == cudaSuccess) e = cudaMalloc(&c->lengths, lengths);
     if (e == cudaSuccess) e = cudaMalloc(&c->tickets, tickets);
-    if (e == cudaSuccess) e = cudaMalloc(&c->partial, (size_t)kKv8MaxCtas * kKv8MaxRows * (head_dim + 2) * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&c->partial, (size_t)kKv8MaxParts * kKv8MaxRows * (head_dim + 2) * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&c->wide, wide);
     if (e == cudaSuccess) e = cudaMalloc(&c->factors, blocks_of_one * sizeof(float4));
     // Codes and scales are read only after they have been written; rows of an open block past its length are

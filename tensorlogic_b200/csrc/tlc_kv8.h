@@ -21,8 +21,9 @@
 #include "tlc_internal.h"
 
 constexpr int kKv8Block = 64;     // positions per block
-constexpr int kKv8MaxCtas = 640;  // CTAs of a launch that shares keys over CTAs (they need workspace)
-constexpr int kKv8MaxRows = 16;   // (query, head) rows per CTA of such a launch
+constexpr int kKv8MaxCtas = 640;  // CTAs of a launch that shares keys over several clusters of eight
+constexpr int kKv8MaxParts = kKv8MaxCtas / 8;  // what they leave in the workspace: a part for each cluster
+constexpr int kKv8MaxRows = 16;                // (query, head) rows of a part
 constexpr int kKv8Tickets = 1024;
 
 struct tlc_kvcache8 {
@@ -33,7 +34,7 @@ struct tlc_kvcache8 {
     float *scales;    // [layer][sequence][kv head][block][K, V]
     __half *open;     // [layer][sequence][kv head][K, V][64 * D], fragment order
     int *lengths;     // [layer][sequence][kv head][K, V]: rows held (a copy for each CTA that appends)
-    float *partial;   // shared keys: [CTA][row][D + 2]
+    float *partial;   // of several clusters: maximum and sum [kKv8MaxParts * kKv8MaxRows][2], then O [..][D]
     int *tickets;     // zero between launches
     // For long prompts: the blocks of one layer and sequence as f16 rows [K, V][kv head][position][D], and per block what
     // they count (kv8_widen).  Made with the cache, so that no prompt allocates, in a stream capture or out of it.

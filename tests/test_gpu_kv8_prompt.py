@@ -294,3 +294,14 @@ def test_first_prompt_in_a_capture(dev, H, Hkv, D):
     dev.synchronize()
     assert dev.mem_info()[0] == free
     assert same(out.cpu().numpy(), got)
+
+
+def test_bytes_of_a_small_cache(dev):
+    """What a cache of 64 rows allocates is its workspace: one part for each cluster that leaves a part, below 2 MB."""
+    from tensorlogic_b200.api import KVCache8
+    dev.synchronize()
+    free = dev.mem_info()[0]
+    held = [KVCache8(dev, 1, 1, 128, max_seq=64) for _ in range(16)]
+    dev.synchronize()
+    assert free - dev.mem_info()[0] <= 16 * 2**21
+    del held
