@@ -737,8 +737,7 @@ extern "C" int32_t tlc_attention8(tlc_ctx *ctx, tlc_kvcache8 *cache, int32_t lay
     TLC_REQUIRE(items <= INT_MAX, TLC_ERR_INVALID_DIMENSION, "attention8: %d sequences of %d queries", batch, n_queries);
     p.items = (int)items;
     const double t = share_out(ctx, D, nt, (int)((T + kKv8Block - 1) / kKv8Block), p);
-    const bool tc = ctx->attn8_tc == 0 ? batch * tcgen05_us(ctx, D, Hkv, G, n_queries, q_pos0) < t : ctx->attn8_tc == 1;
-    if (n_queries > 1 && G <= 128 && tc) {
+    if (n_queries > 1 && G <= 128 && (ctx->attn8_tc == 0 ? batch * tcgen05_us(ctx, D, Hkv, G, n_queries, q_pos0) < t : ctx->attn8_tc == 1)) {
         for (int b = 0; b < batch; b++) {  // through one image, a sequence at a time
             const size_t at = (size_t)b * n_queries * n_heads * D;
             if (int32_t rc = kv8_attention_tc(ctx, cache, layer, sequence + b, static_cast<const __half *>(q_dev) + at,

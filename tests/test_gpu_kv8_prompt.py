@@ -107,14 +107,16 @@ def test_prompt(dev, form, H, Hkv, D, I, pos0):
     dev.synchronize()
 
 
-def test_groups_too_large_for_a_tile(dev):
+@pytest.mark.parametrize("asked", [0, 1])
+@pytest.mark.parametrize("I", [1, 70])
+def test_groups_too_large_for_a_tile(dev, asked, I):
     from tensorlogic_b200.api import KVCache8
-    H, Hkv, D, I = 129, 1, 64, 70
+    H, Hkv, D = 129, 1, 64
     k, v = rows(1, I, Hkv, D)
     q = queries(1, I, H, D)
     cache = KVCache8(dev, 1, Hkv, D, max_seq=I)
     cache.append(0, dev.tensor(k), dev.tensor(v))
-    with forced(dev, 1):
+    with forced(dev, asked):
         got = prompt(dev, cache, q, H, 2)
     check_attention(got, q, exact_values(k), exact_values(v), 0)
     dev.synchronize()
