@@ -652,9 +652,12 @@ int32_t launch(tlc_ctx *ctx, const Params &p) {
 
 // Warps that share an item of `units` blocks -- 1, 2, 4, or four in each of 2, 4, 8 or a multiple of eight CTAs: the
 // fewest microseconds of
-//   blocks of a warp x (the larger of a block's latency and its share of the SM, 44 KB/us for its warps),
-// as often as the SM's warps have to be filled, and the merge, in shared memory, in a cluster, or of clusters.  (Clusters of
-// eight lie in one part of the chip: beyond two for nine SMs they leave some SMs with more CTAs than others.)
+//   blocks of a warp x (the larger of a block's latency and its share of the SM, 44 KB/us for its warps), and the merge
+//   -- in shared memory, in a cluster, or of clusters --
+// as often as the SM's warps have to be filled.  (Clusters of eight lie in one part of the chip: beyond two for nine SMs they
+// leave some SMs with more CTAs than others.)
+// 2048 queries, 32 heads of 128, fill them several times over: one warp an item takes 187 us, two (the rule's) 207, four 228,
+// eight 369, 32 1204.
 // One query, 32 heads on four of 64, behind 40000 positions takes 14.2 us with 64 warps to a KV head, 11.9 with 128, 12.5
 // with 256, 16.2 with 576; behind 130000 30, 22, 17 and 21.
 // Sixteen queries behind 1000 positions, 32 heads of 128: one warp 28.5 us, two 19.8, four 12.8, sixteen 11.8; 192
@@ -672,7 +675,8 @@ double share_out(const tlc_ctx *ctx, int D, int nt, int units, Params &p) {
                                                                     : ((long long)p.items * w + ctx->sm_count - 1) / ctx->sm_count;
         const long long rounds = (per_sm + warps - 1) / warps;
         const double at_once = (double)(per_sm < warps ? per_sm : warps), block = latency > at_once * share ? latency : at_once * share;
-        const double t = (double)rounds * ((units + w - 1) / w) * block + (w == 1 ? 0.0 : w <= kWarps ? 0.7 : nsplit <= 8 ? 1.5 : 3.0 + 0.12 * (nsplit / 8));
+        const double merge = w == 1 ? 0.0 : w <= kWarps ? 0.7 : nsplit <= 8 ? 1.5 : 3.0 + 0.12 * (nsplit / 8);
+        const double t = (double)rounds * ((units + w - 1) / w * block + merge);
         if (t < best) {
             best = t;
             p.warps = w < kWarps ? w : kWarps;

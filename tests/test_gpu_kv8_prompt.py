@@ -307,3 +307,33 @@ def test_bytes_of_a_small_cache(dev):
     dev.synchronize()
     assert free - dev.mem_info()[0] <= 16 * 2**21
     del held
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(32, 32, 128), (32, 4, 64), (160, 1, 64)])
+def test_many_items_are_not_cut_finer(dev, H, Hkv, D):
+    """Twice the prompt is four times the work.  Where warps are filled many times over, an item stays with few of them: its
+    results are merged each time, not once."""
+    import torch
+    from tensorlogic_b200.api import KVCache8
+    T = 2048
+    cache = KVCache8(dev, 1, Hkv, D, max_seq=T)
+    k, v = rows(1, T, Hkv, D)
+    cache.append(0, dev.tensor(k), dev.tensor(v))
+    stream = torch.cuda.ExternalStream(dev.stream)
+
+    def took(I):
+        q = dev.tensor(queries(1, I, H, D))
+        times = []
+        for _ in range(6):
+            with torch.cuda.stream(stream):
+                start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                start.record()
+                cache.attention(0, q, H)
+                end.record()
+            dev.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    with forced(dev, 2):  # (the third group is too large for the other kernel anyway)
+        assert took(T) <= 8 * took(T // 2)
+    dev.synchronize()
