@@ -10,7 +10,9 @@
 // alone:
 //   S^T = K.Q^T  16 keys x 8 rows a product, codes as the 16-row operand (PRMT makes it, tlc_kv8.h)
 //   P            f32 maximum and sums over the keys of a row, P rounded to f16, times 2^12 so that small
-//                probabilities keep their bits; the sum is of the rounded values
+//                probabilities keep their bits; the sum is of the rounded values.  (The product's operands are f16, and
+//                P in two of them would be the product twice over: against 64 bits the output is off by 2.4e-4 to
+//                3e-4, by 2.1e-4 from its own rounding alone.  The codes are off by up to 2^-8 of their block's largest.)
 //   O^T += V^T.P P turned over by movmatrix, f32 accumulators of the block, scaled by s_v when they join O
 // A warp's blocks arrive by cp.async in a ring of its own; a lane copies the very bytes it will use, so a warp needs no
 // barrier and no other lane until the results of an item's warps are merged in shared memory.  CTAs that share its keys
@@ -20,7 +22,7 @@
 //
 // Many sequences: bound by HBM while all warps have blocks (32 sequences of about 600 keys, 32 heads of 128: 33 us, 157 MB
 // at 0.72 of the copy's rate; the tensor pipe is 15 % busy).  One sequence: by latency, 1.0 us a block and warp, and the
-// merge (65000 keys, 4 KV heads of 64: 12.5 us; 512 keys 5.5, of which a call's launch is 3.6).
+// merge (65000 keys, 4 KV heads of 64: 13.5 us, 12.3 where the L2 holds them; 512 keys 5.5, of which a call's launch is 3.6).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -658,10 +660,10 @@ int32_t launch(tlc_ctx *ctx, const Params &p) {
 // leave some SMs with more CTAs than others.)
 // 2048 queries, 32 heads of 128, fill them several times over: one warp an item takes 187 us, two (the rule's) 207, four 228,
 // eight 369, 32 1204.
-// One query, 32 heads on four of 64, behind 40000 positions takes 14.2 us with 64 warps to a KV head, 11.9 with 128, 12.5
-// with 256, 16.2 with 576; behind 130000 30, 22, 17 and 21.
-// Sixteen queries behind 1000 positions, 32 heads of 128: one warp 28.5 us, two 19.8, four 12.8, sixteen 11.8; 192
-// queries: 49.2, 31.9, 35.6, 68.
+// One query, 32 heads on four of 64, behind 40000 positions takes 14.2 us with 64 warps to a KV head, 11.7 with 128, 10.9
+// with 256, 16.2 with 576; behind 130000 32, 23, 19 and 23.
+// Sixteen queries behind 1000 positions, 32 heads of 128: one warp 29.9 us, two 21.0, four 13.7, sixteen 11.3; 192
+// queries: 49.5, 31.9, 35.9, 68.
 double share_out(const tlc_ctx *ctx, int D, int nt, int units, Params &p) {
     const double latency = D == 64 ? nt == 1 ? 0.85 : 1.05 : nt == 1 ? 1.2 : 1.6, share = kKv8Block * D * 2 / 44e3;
     const int warps = kWarps * places(D, nt);  // of an SM
@@ -688,8 +690,8 @@ double share_out(const tlc_ctx *ctx, int D, int nt, int units, Params &p) {
 }
 // Microseconds that the tcgen05 form takes more than a launch of the other one: another launch and the longer start of its
 // CTAs, the image of the blocks (three bytes moved a value), and its tiles of 128 rows x 64 keys, by the longest CTA or by
-// what an SM gets through.  32 heads of 128: 192 queries 12.1 us here, 8.6 there, behind 1000 positions 31.9 and 23.5;
-// 64 behind 1000 15.2 and 24.5.  2048 queries 225 and 51.
+// what an SM gets through.  32 heads of 128: 192 queries 12.3 us here, 8.8 there, behind 1000 positions 31.6 and 22.7;
+// 64 behind 1000 15.2 and 24.7.  2048 queries 207 and 48.
 double tcgen05_us(const tlc_ctx *ctx, int D, int Hkv, int G, int I, int pos0) {
     const int rq = 128 / G, tiles = (I + rq - 1) / rq, units = (pos0 + I + kKv8Block - 1) / kKv8Block;
     const double image = (double)units * Hkv * kKv8Block * D * 6 / 5e6, longest = units * (D == 64 ? 0.45 : 0.55);

@@ -7,13 +7,17 @@
 //   S = Q.C_k^T   Q and codes in shared memory (TMA, 128-byte swizzle), f32 in tensor memory
 //   softmax       one row per thread: x = S s_k scale log2(e) + log2(s_v), P = 2^(x - m + 8) in f16, where m follows the
 //                 row's largest x only when that has risen by more than 2^7 (P stays below 2^15): the block's
-//                 factor of V is part of P, its sum is divided by it again
+//                 factor of V is part of P, its sum is divided by it again.  The sum is of P before it is rounded: a block
+//                 of small values has little of P, which f16 may cut off, but all its part of the sum.  (f16 because the
+//                 product's operands are: against 64 bits the output is off by 2.6e-4 to 2.7e-4, by 2.1e-4 from its own
+//                 rounding alone.)  The open block's values are their own codes, factor 1, however small they are: it
+//                 comes last, so that what it lifts m by is taken from sums in f32, not from P of a later block.
 //   O += P.C_v    P from tensor memory, over the scores it was made from; codes of V as [key][d], the N-major operand
 //
 // Warps:  0  Q, K and V by TMA      1  tensor memory and MMA issue      2-5  softmax, rescale, output
 //
 // Bound by the tiles' way out of the L2: 2048 queries, 32 heads of 128 move 285 MB there in 41 us (7 TB/s; tensor pipe
-// 45 %, as a product of 64 keys takes as long as one of 128), behind 11 us for the image: 55 us a call.  One CTA with twice
+// 45 %, as a product of 64 keys takes as long as one of 128), behind 11 us for the image: 54 us a call.  One CTA with twice
 // the rows moves half of it and took 55 to 61 us a call, its softmax in turn with its own products.
 //
 // All waits are bounded; one that runs out sets the status word and lets the CTA drain, free its tensor memory and
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // The last queries see the most keys: their tiles go first.
     const int hk = blockIdx.x % p.n_kv_heads, qt = p.q_tiles - 1 - blockIdx.x / p.n_kv_heads;
     const int G = p.G, RQ = p.RQ;
-    const int keys = min(p.lengths[2 * hk], p.pos0 + p.I);  // (fewer than the queries' own: said by the host's caller below)
+    const int keys = min(p.lengths[2 * hk], p.pos0 + p.I);  // (fewer than the queries' own: said below)
     const int k_end = min(keys, p.pos0 + min(p.I, (qt + 1) * RQ));
     const int n = (k_end + kKeys - 1) / kKeys;
     if (tid == 0 && qt == 0 && keys < p.pos0 + p.I && atomicCAS(&p.status->code, 0, TLC_DEV_INDEX) == 0) p.status->where = 400;

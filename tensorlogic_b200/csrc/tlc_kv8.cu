@@ -119,9 +119,10 @@ __device__ __forceinline__ int turn_d(int lane) { return 8 * (lane >> 4); }
 // so that old rows (16 bytes a lane) and codes (512 a warp) are read and written as they are.  K's order takes eight
 // neighbouring values of a row, which is how new rows come too; V's takes four keys of a value, and new rows are turned
 // by ldmatrix.  Rows of an open block go the same way, 16 keys a warp; fewer than four, or behind older ones, one by one.
-// Bound by the rows' bytes and, for few of them, by the launch: 2048 rows of 32 heads of 128 take 13.4 us (3.8 TB/s), 300
-// of them 6.3, 60 3.2 (8.2 and 5.0 with the open block one by one behind the first; the launch alone is 3.1), and 2048
-// with their read-back 22.9 against 53 for a form that went through shared memory value by value.
+// Bound by the rows' bytes and, for few of them, by the launch: 2048 rows of 32 heads of 128 take 15.4 us (3.3 TB/s; 14.0
+// where the L2 holds the rows already), 300 of them 6.7, 60 3.2 (8.2 and 5.0 with the open block one by one behind the first;
+// the launch alone is 3.1), and 2048 with their read-back 25.0 against 53 for a form that went through shared memory value
+// by value.
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
     constexpr int PITCH = D + 8, PIECES = D / 8, C = D / 32;

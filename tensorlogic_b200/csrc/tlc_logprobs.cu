@@ -325,7 +325,7 @@ __device__ __forceinline__ void ranked(const K *keys, int n, int top, F &&take) 
 // With alternatives.  Bound by latencies: of a turn's 8000 cycles (1 x 100003 split eight ways) 1500 pass until the
 // logits are there, 1200 in the exponentials (16384, at 16 a cycle of the SM), the rest between barriers -- bound,
 // candidates, ranks -- and 2000 more in joining the cluster, 1700 in ranking what its CTAs found.  512 threads halve
-// the steps of each against 256 and leave room for a second CTA on the SM.  1 x 32000 with 5 alternatives takes 4.7 us, of
+// the steps of each against 256 and leave room for a second CTA on the SM.  1 x 32000 with 5 alternatives takes 4.8 us, of
 // which a call's launch is 3.6; 37 x 100003 with 20 11.2 (seven CTAs a row: all 37 clusters find room at once).
 template <int PIECES>
 __global__ void __launch_bounds__(kTopThreads, 2) logprob_top_kernel(const LogprobParams p) {
@@ -582,7 +582,8 @@ cudaError_t launch_top(tlc_ctx *ctx, cudaLaunchConfig_t &cfg, const LogprobParam
 // How many 16-byte pieces a slice has, at most.
 constexpr int slice_pieces(int vocab, int ctas) { return (int)((((long long)vocab + 14) / 8 + ctas - 1) / ctas); }
 
-// How many clusters of c CTAs of the kernel with alternatives run at once, two CTAs an SM.
+// How many clusters of c CTAs of the kernel with alternatives run at once, two CTAs an SM.  The plan takes it as the measure of
+// the GPU's room for rows without alternatives too: their CTAs are half as large, and the costs below were fitted with it.
 int resident_clusters(tlc_ctx *ctx, int c) {
     static int known[64][kMaxCluster + 1] = {};
     int &n = known[ctx->device & 63][c];
@@ -609,8 +610,11 @@ int resident_clusters(tlc_ctx *ctx, int c) {
 // row.  A row costs the joining of its CTAs and a CTA's work: a turn of 2048 pieces with alternatives (3.45, with 512 or
 // 1024 pieces 2 or 2.5), 15000 logits a microsecond without.  Half of the clusters that run at once find SMs of their own
 // (of more than two CTAs, which lie in one part of the chip, a quarter); all of them take 1.5 times as long, more wait.
-// With 20 alternatives 36 x 32000 takes 9.2, 6.6, 8.5, 7.4, 7.5, 7.7, 8.7 and 9.9 us with 1 to 8 CTAs a row, 36 x 100003
-// 27.3, 17.8, 14.0, 13.9, 13.8, 13.4, 10.1 and 12.3, 148 x 100003 30.4, 25.1, 35.6, 32.5, 37.2, 43.0, 29.8 and 32.8.
+// With 20 alternatives 36 x 32000 takes 9.2, 6.6, 6.8, 7.4, 7.5, 7.8, 8.6 and 10.0 us with 1 to 8 CTAs a row (two are taken),
+// 36 x 100003 27.3, 17.7, 13.9, 14.0, 13.7, 13.5, 9.7 and 12.3 (seven), 148 x 100003 27.7, 24.4, 35.0, 31.1, 36.2, 41.7, 29.0
+// and 31.9 (two).  Without, 36 x 100003 takes 8.5, 6.6, 5.7, 6.0, 6.6, 5.9, 5.8 and 7.1 (seven), 148 x 100003 8.6, 9.1, 11.2,
+// 11.8, 12.0, 13.3, 12.1 and 14.0 (two), 512 x 32000 8.8, 11.3, 15.9, 15.1, 18.1, 21.2, 24.2 and 27.7 (one).  Of 128 pairs of rows and vocabulary the
+// plan is up to 18 % behind the best number, and 31 % once (16 x 151936 with alternatives).
 int ctas_a_row(tlc_ctx *ctx, int rows, int vocab, bool alternatives) {
     constexpr double kJoin[2][kMaxCluster] = {{0, 1.1, 1.2, 1.3, 1.5, 1.7, 1.9, 2.1}, {0, 1.2, 1.3, 1.4, 1.45, 1.5, 1.55, 1.6}};
     int best = 1;
