@@ -604,7 +604,7 @@ class KVCache8:
         held = self.lengths[layer, sequence:]
         pos_t = None
         if positions is None:
-            at = int(held[0]) if position is None else int(position)
+            at = int(held[0]) if position is None else int(_whole(position)[0])
             if not 0 <= at <= held[0]:
                 raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {at}, size {held[0]}")
         else:
@@ -644,9 +644,12 @@ class KVCache8:
         self._check(layer, sequence, batch, q)
         nq = q.size // (n_heads * D * batch)
         held = self.lengths[layer, sequence:sequence + batch]
+        q_pos0 = int(_whole(q_pos0)[0])
         pos_t, max_keys = None, q_pos0 + nq
         if positions is None:
             wrong = held < q_pos0 + nq
+            if q_pos0 < 0:  # (before 32 bits make something else of it)
+                raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {q_pos0}, size {held[0]}")
             if wrong.any():
                 raise TensorError(_lib.ERR_INDEX, f"Index out of bounds: index {q_pos0 + nq - 1}, size {held[wrong][0]}")
         else:

@@ -159,3 +159,18 @@ def test_tokens_of_any_integer_type(fake, monkeypatch):
     for t in (np.int8, np.uint8, np.int64, np.uint64):
         token_logprobs(_tensor(fake, (2, 10)), np.array([3, 9], t))
     assert all(a.dtype == np.int32 and list(a) == [3, 9] for a in sent) and len(sent) == 4
+
+
+@pytest.mark.parametrize("wrong", [-1, -2**32, -2**32 + 3, 2**32, 2.5])
+def test_a_single_position_is_checked_whole_too(fake, wrong):
+    cache = KVCache8(fake, 1, 2, 64, max_seq=100)
+    rows = _tensor(fake, (5, 2, 64))
+    cache.append(0, rows, rows)
+    made = len(fake.lib.calls)
+    for call in (lambda: cache.append(0, rows, rows, position=wrong), lambda: cache.attention(0, _tensor(fake, (2, 2, 64)), 2, q_pos0=wrong)):
+        with pytest.raises(_lib.TensorError) as e:
+            call()
+        assert e.value.code == _lib.ERR_INDEX
+    assert len(fake.lib.calls) == made and list(cache.lengths[0]) == [5]
+    cache.append(0, rows, rows, position=np.int64(5))
+    assert list(cache.lengths[0]) == [10]
