@@ -337,3 +337,19 @@ def test_many_items_are_not_cut_finer(dev, H, Hkv, D):
     with forced(dev, 2):  # (the third group is too large for the other kernel anyway)
         assert took(T) <= 8 * took(T // 2)
     dev.synchronize()
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(32, 4, 64), (8, 2, 128)])
+@pytest.mark.parametrize("I,T", [(1, 700), (1, 20000), (60, 700)])
+def test_largest_values_of_a_token(dev, H, Hkv, D, I, T):
+    """The same on the other kernel: one warp, warps, CTAs and clusters that share the keys."""
+    from tensorlogic_b200.api import KVCache8
+    rng = np.random.default_rng(D)
+    k = (rng.standard_normal((T, Hkv, D)) * 0.01).astype(np.float16)
+    q = queries(I, I, H, D)
+    for value in (65504, -65504):
+        v = np.full((T, Hkv, D), value, np.float16)
+        cache = KVCache8(dev, 1, Hkv, D, max_seq=T)
+        cache.append(0, dev.tensor(k), dev.tensor(v))
+        check_attention(prompt(dev, cache, q, H, 2, q_pos0=T - I), q, exact_values(k), exact_values(v), T - I)
+    dev.synchronize()
